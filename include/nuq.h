@@ -212,6 +212,75 @@ int nuq_topk(nuq_context *ctx, const float *logits, uint64_t count, uint32_t k, 
 int nuq_penalize(nuq_context *ctx, float *logits, uint64_t count, const uint32_t *history, uint64_t history_words,
                  float repetition, float presence);
 
+/* The quantised K/V cache of one layer: [pages][kv_heads][page_tokens / 16]
+ * tiles of 16 tokens in device memory, head_dim * (4 * bits + 2) bytes a tile
+ * (nuclis_amd/csrc/cache.h has the byte layout). Values come in groups of 32
+ * along the head dimension with one f16 scale:
+ *   4 bits: m the group's value of largest magnitude (the positive one on a
+ *           tie), d = f16(bf16(clamp(-m / 8, +-2720))), value d * clamp(rint(x / d), -8, 7)
+ *   8 bits: d = f16(min(max|x| / 127 rounded up to 4 significant bits, 56)),
+ *           value d * clamp(rint(x / d), -127, 127)
+ * so every value is an f16 number, and larger ones saturate near 21,760 (4
+ * bits) and 7,112 (8 bits). A token whose K or V in a head holds a non-finite
+ * value is NaN throughout that head: it reads back as NaN and makes NaN the rows
+ * that attend to it, and no others. Token t of page p is slot p * page_tokens
+ * + t. The reference holds its cache in F16 or Q8_0 rows
+ * (inference/src/runtime/session.zig:629-690). */
+typedef struct nuq_cache {
+    uint32_t bits;        /* 4 or 8 */
+    uint32_t page_tokens; /* a power of two, 16 to 4096 */
+    uint32_t kv_heads;    /* 1 to 65535 */
+    uint32_t head_dim;    /* 64, 128 or 256 */
+    uint64_t pages;
+    void *bytes;          /* device, 16-byte aligned */
+    uint64_t byte_len;    /* nuq_cache_bytes of the other fields */
+} nuq_cache;
+/* Bytes a cache of these sizes takes (`bytes` and `byte_len` are not read);
+ * InvalidShape for sizes it cannot have. Host only. */
+int nuq_cache_bytes(const nuq_cache *cache, uint64_t *bytes);
+/* Quantises `tokens` tokens' keys and values into their slots. k and v are
+ * [tokens][kv_heads][head_dim] of `dtype` (F32 or F16), rows `k_stride` /
+ * `v_stride` elements apart, each row 16-byte aligned. slots is a device array;
+ * a slot outside the cache (-1 for padding) skips its token; slots of one call
+ * are distinct. */
+int nuq_cache_write(nuq_context *ctx, const nuq_cache *cache, const void *k, const void *v, uint32_t dtype,
+                    uint64_t k_stride, uint64_t v_stride, const int64_t *slots, uint64_t tokens);
+/* Reads tokens back as F32 or F16 (both exact); zeros for a slot outside the
+ * cache. k and v as for nuq_cache_write. */
+int nuq_cache_read(nuq_context *ctx, const nuq_cache *cache, const int64_t *slots, uint64_t tokens, uint32_t dtype,
+                   void *k, void *v, uint64_t k_stride, uint64_t v_stride);
+/* Causal attention of new tokens over the cache, o = softmax(scale q K^T) V.
+ * Sequence b holds lengths[b] tokens in the pages page_table[b] names in order;
+ * its new tokens are the last of them (written before this call) and have the
+ * query rows [starts[b], starts[b + 1]), or max_tokens rows each where starts
+ * is null. The query at position p sees the cached positions j <= p, with a
+ * window also j > p - window. q and out are [rows][q_heads][head_dim] of `dtype`,
+ * 16-byte aligned rows; query head i reads KV head i / (q_heads / kv_heads).
+ * F32 queries are served at F32 precision; F16 ones with F32 scores, sums and
+ * outputs and weights rounded to f16 once. Rows that see nothing are zeros;
+ * positions on a page outside [0, pages) are not attended to; lengths past the
+ * table are cut to it; rows of `out` that no sequence has stay as they are. */
+typedef struct nuq_attention {
+    const void *q;
+    void *out;
+    uint32_t dtype;             /* of q and out: NUQ_F32 or NUQ_F16 */
+    uint32_t q_heads;           /* a multiple of kv_heads */
+    uint64_t q_stride;          /* elements from a row to the next */
+    uint64_t out_stride;
+    uint64_t rows;              /* query rows in all */
+    const int32_t *page_table;  /* device [batch][table_stride] */
+    uint64_t table_stride;
+    uint64_t table_width;       /* entries of a row that may be read */
+    const int32_t *lengths;     /* device [batch] */
+    const int32_t *starts;      /* device [batch + 1], or null */
+    uint32_t batch;
+    uint32_t max_tokens;        /* most new tokens of a sequence; rows past it are not computed */
+    uint64_t max_length;        /* most tokens a sequence holds, for the split of the work; 0: the table's */
+    float scale;                /* of the scores: positive and finite */
+    uint32_t window;            /* 0: none */
+} nuq_attention;
+int nuq_cache_attention(nuq_context *ctx, const nuq_cache *cache, const nuq_attention *args);
+
 /* Weight preparation on the host (not part of the reference's backend):
  * quantize `rows` F32 rows of `columns` into GGUF rows in dst (host memory,
  * dst_len = rows * row bytes). Q8_0 is quant/encode.zig:17-36 exactly; the

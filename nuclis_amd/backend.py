@@ -99,6 +99,21 @@ class TopK:
     finite: bool
 
 
+class _Cache(ctypes.Structure):
+    _fields_ = [("bits", ctypes.c_uint32), ("page_tokens", ctypes.c_uint32), ("kv_heads", ctypes.c_uint32),
+                ("head_dim", ctypes.c_uint32), ("pages", ctypes.c_uint64), ("bytes", ctypes.c_void_p),
+                ("byte_len", ctypes.c_uint64)]
+
+
+class _Attention(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("out", ctypes.c_void_p), ("dtype", ctypes.c_uint32),
+                ("q_heads", ctypes.c_uint32), ("q_stride", ctypes.c_uint64), ("out_stride", ctypes.c_uint64),
+                ("rows", ctypes.c_uint64), ("page_table", ctypes.c_void_p), ("table_stride", ctypes.c_uint64),
+                ("table_width", ctypes.c_uint64), ("lengths", ctypes.c_void_p), ("starts", ctypes.c_void_p),
+                ("batch", ctypes.c_uint32), ("max_tokens", ctypes.c_uint32), ("max_length", ctypes.c_uint64),
+                ("scale", ctypes.c_float), ("window", ctypes.c_uint32)]
+
+
 class _Segment(ctypes.Structure):
     _fields_ = [("matrix", _Matrix), ("output", ctypes.c_void_p)]
 
@@ -110,7 +125,7 @@ EXPORTS = [
     "nuq_validate_row", "nuq_embed", "nuq_dequant_range", "nuq_matvec", "nuq_matvec_rows", "nuq_matmul",
     "nuq_matmul_kernel", "nuq_matvec_segments", "nuq_argmax", "nuq_quantize_rows", "nuq_dequant_rows", "nuq_gemv",
     "nuq_gemm", "nuq_topk", "nuq_penalize", "nuq_reserve_workspace", "nuq_workspace_bytes",
-    "nuq_matvec_segments_noalloc",
+    "nuq_matvec_segments_noalloc", "nuq_cache_bytes", "nuq_cache_write", "nuq_cache_read", "nuq_cache_attention",
 ]
 
 
@@ -151,6 +166,11 @@ def lib() -> ctypes.CDLL:
         L.nuq_matvec_segments_noalloc.argtypes = [vp, ctypes.POINTER(_Segment), u32, vp, u32]
         L.nuq_argmax.argtypes = [vp, vp, u64, ctypes.POINTER(u32)]
         L.nuq_quantize_rows.argtypes = [u32, vp, u64, u64, vp, u64]
+        cp = ctypes.POINTER(_Cache)
+        L.nuq_cache_bytes.argtypes = [cp, ctypes.POINTER(u64)]
+        L.nuq_cache_write.argtypes = [vp, cp, vp, vp, u32, u64, u64, vp, u64]
+        L.nuq_cache_read.argtypes = [vp, cp, vp, u64, u32, vp, vp, u64, u64]
+        L.nuq_cache_attention.argtypes = [vp, cp, ctypes.POINTER(_Attention)]
         _lib = L
     return _lib
 
@@ -205,6 +225,37 @@ class Matrix:
     def c(self) -> _Matrix:
         n = self.byte_len if self.byte_len is not None else self.bytes.numel() * self.bytes.element_size()
         return _Matrix(self.encoding, 0, self.rows, self.columns, self.bytes.data_ptr(), n)
+
+
+def cache_bytes(bits: int, pages: int, page_tokens: int, kv_heads: int, head_dim: int) -> int:
+    """Device bytes of a KVCache of these sizes."""
+    n = ctypes.c_uint64(0)
+    for value in (bits, page_tokens, kv_heads, head_dim):
+        if not 0 <= value < 1 << 32:
+            raise InvalidShape(f"InvalidShape: {value}")
+    _raise(lib().nuq_cache_bytes(ctypes.byref(_Cache(bits, page_tokens, kv_heads, head_dim, pages, None, 0)),
+                                 ctypes.byref(n)))
+    return n.value
+
+
+class KVCache:
+    """The quantised K/V cache of one layer (nuq_cache, include/nuq.h): `pages`
+    pages of `page_tokens` tokens, 4 or 8 bits. Token t of page p is slot
+    p * page_tokens + t. `bytes` is a contiguous uint8 CUDA tensor of
+    cache_bytes(...) bytes; by default a new one of zeros."""
+
+    def __init__(self, bits: int, pages: int, page_tokens: int, kv_heads: int, head_dim: int, bytes=None, device=0):
+        self.bits, self.pages, self.page_tokens = bits, pages, page_tokens
+        self.kv_heads, self.head_dim = kv_heads, head_dim
+        if bytes is None:
+            import torch
+            bytes = torch.zeros(cache_bytes(bits, pages, page_tokens, kv_heads, head_dim), dtype=torch.uint8,
+                                device=f"cuda:{device}")
+        elif not bytes.is_contiguous():
+            raise InvalidShape("InvalidShape: the cache's bytes are not contiguous")
+        self.bytes = bytes
+        self._c = _Cache(bits, page_tokens, kv_heads, head_dim, pages, bytes.data_ptr(),
+                         bytes.numel() * bytes.element_size())
 
 
 def _ptr(t) -> int | None:
@@ -334,6 +385,81 @@ class Backend:
             total += partial
         return TopK(temperature, [int(i) & 0xffffffff for i in indices.cpu().tolist()[:k]],
                     values.cpu().tolist()[:k], total, not bool(flags.cpu().any()))
+
+    # -- the quantised cache and the attention over it ------------------------
+    def _index(self, t, dtype, name: str):
+        """A contiguous index tensor's address."""
+        if t.dtype is not dtype:
+            raise InvalidArgument(f"{name} must be {dtype}, not {t.dtype}")
+        if not t.is_contiguous():
+            raise InvalidShape(f"InvalidShape: {name} is not contiguous")
+        return t.data_ptr()
+
+    def _heads(self, t, heads: int, head_dim: int, name: str) -> int:
+        """Checks [rows][heads][head_dim] with contiguous rows; the dtype's code."""
+        if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != head_dim:
+            raise InvalidShape(f"InvalidShape: {name} is {tuple(t.shape)}, not [rows][{heads}][{head_dim}]")
+        stride = t.stride()
+        if stride[2] != 1 or (heads > 1 and stride[1] != head_dim):
+            raise InvalidShape(f"InvalidShape: {name}'s rows are not contiguous")
+        if t.dtype is self._torch.float32:
+            return F32
+        if t.dtype is self._torch.float16:
+            return F16
+        raise InvalidArgument(f"{name} is {t.dtype}, not float32 or float16")
+
+    def _slots(self, cache: KVCache, k, v, slots):
+        dtype = self._heads(k, cache.kv_heads, cache.head_dim, "k")
+        if self._heads(v, cache.kv_heads, cache.head_dim, "v") != dtype:
+            raise InvalidArgument("k and v differ in dtype")
+        tokens = slots.numel()
+        if k.shape[0] != tokens or v.shape[0] != tokens:
+            raise InvalidShape(f"InvalidShape: {tokens} slots for {k.shape[0]} keys and {v.shape[0]} values")
+        return dtype, tokens, self._index(slots, self._torch.int64, "slots")
+
+    def cache_write(self, cache: KVCache, k, v, slots) -> None:
+        """Quantises tokens' keys and values [tokens][kv_heads][head_dim] (F32
+        or F16; rows may be strided) into their slots (int64; -1 skips)."""
+        dtype, tokens, at = self._slots(cache, k, v, slots)
+        self._call(lib().nuq_cache_write, ctypes.byref(cache._c), k.data_ptr(), v.data_ptr(), dtype, k.stride(0),
+                   v.stride(0), at, tokens)
+
+    def cache_read(self, cache: KVCache, slots, k, v) -> None:
+        """Reads slots back into k and v (F32 or F16, both exact)."""
+        dtype, tokens, at = self._slots(cache, k, v, slots)
+        self._call(lib().nuq_cache_read, ctypes.byref(cache._c), at, tokens, dtype, k.data_ptr(), v.data_ptr(),
+                   k.stride(0), v.stride(0))
+
+    def cache_attention(self, cache: KVCache, q, output, page_table, lengths, starts=None, scale: float | None = None,
+                        window: int = 0, max_tokens: int | None = None, max_length: int = 0) -> None:
+        """Causal attention of new tokens' queries [rows][q_heads][head_dim]
+        over the cache (nuq_cache_attention, include/nuq.h). page_table int32
+        [batch][pages], lengths int32 [batch] (the new tokens among them), starts
+        int32 [batch + 1] where the sequences bring different counts of rows.
+        `scale` is head_dim ** -0.5 by default; `max_tokens` (a bound on a
+        sequence's rows) and `max_length` (on its tokens) size the launch."""
+        if q.dim() != 3:
+            raise InvalidShape(f"InvalidShape: q is {tuple(q.shape)}, not [rows][q_heads][head_dim]")
+        rows, heads = q.shape[0], q.shape[1]
+        dtype = self._heads(q, heads, cache.head_dim, "q")
+        if self._heads(output, heads, cache.head_dim, "output") != dtype or output.shape[0] != rows:
+            raise InvalidShape("InvalidShape: the output is not of q's shape and dtype")
+        int32 = self._torch.int32
+        batch = lengths.numel()
+        if page_table.dim() != 2 or page_table.shape[0] != batch:
+            raise InvalidShape(f"InvalidShape: page table {tuple(page_table.shape)} for {batch} sequences")
+        if page_table.dtype is not int32 or page_table.stride(1) != 1:
+            raise InvalidArgument("the page table is not int32 with contiguous rows")
+        if starts is not None and starts.numel() != batch + 1:
+            raise InvalidShape(f"InvalidShape: {starts.numel()} starts for {batch} sequences")
+        if max_tokens is None:
+            max_tokens = rows if starts is not None else rows // max(batch, 1)
+        args = _Attention(q.data_ptr(), output.data_ptr(), dtype, heads, q.stride(0), output.stride(0), rows,
+                          page_table.data_ptr(), page_table.stride(0), page_table.shape[1],
+                          self._index(lengths, int32, "lengths"),
+                          None if starts is None else self._index(starts, int32, "starts"), batch, max_tokens,
+                          max_length, cache.head_dim ** -0.5 if scale is None else scale, window)
+        self._call(lib().nuq_cache_attention, ctypes.byref(cache._c), ctypes.byref(args))
 
     def argmax(self, logits) -> int:
         idx = ctypes.c_uint32(0)

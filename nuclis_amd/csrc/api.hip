@@ -26,6 +26,7 @@
 #include "../../include/nuq.h"
 #include "../../include/nuq_gguf.h"
 #include "gguf_doc.h"
+#include "attention.h"
 #include "formats.h"
 #include "kernels.h"
 
@@ -341,6 +342,63 @@ int matmul_impl(nuq_context *ctx, uint32_t kernel, const nuq_matrix *m, const vo
                                       (uint32_t)m->columns, x, f16, in_stride, out, out_stride, tokens, plan,
                                       ctx->split),
                      "tile launch");
+}
+
+// Bytes of a cache, 0 for sizes it cannot have (or that pass 2^63).
+uint64_t cache_bytes(const nuq_cache *c) {
+    if (c->bits != 4 && c->bits != 8) return 0;
+    if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return 0;
+    if (c->page_tokens < 16 || c->page_tokens > 4096 || (c->page_tokens & (c->page_tokens - 1)) != 0) return 0;
+    if (c->kv_heads == 0 || c->kv_heads > 65535 || c->pages == 0 || c->pages > 0x7fffffffull) return 0;
+    // at most 2^31 * 2^16 * 2^8 * 2^14 = 2^69 in theory: divide before multiplying
+    const uint64_t page = (uint64_t)c->kv_heads * (c->page_tokens / 16) * nuq::cache_tile_bytes(c->bits, c->head_dim);
+    return c->pages > (1ull << 63) / page ? 0 : c->pages * page;
+}
+
+int check_cache(nuq_context *ctx, const nuq_cache *c, nuq::CacheView *view) {
+    if (!c) return fail(ctx, NUQ_INVALID_ARGUMENT, "null cache");
+    const uint64_t bytes = cache_bytes(c);
+    if (bytes == 0)
+        return fail(ctx, NUQ_INVALID_SHAPE, "cache of %u bits, %u tokens a page, %u heads of %u, %llu pages", c->bits,
+                    c->page_tokens, c->kv_heads, c->head_dim, (unsigned long long)c->pages);
+    if (!c->bytes) return fail(ctx, NUQ_INVALID_ARGUMENT, "null cache bytes");
+    if (c->byte_len != bytes)
+        return fail(ctx, NUQ_INVALID_BYTE_LENGTH, "InvalidByteLength: cache of %llu bytes, %llu expected",
+                    (unsigned long long)c->byte_len, (unsigned long long)bytes);
+    if ((uintptr_t)c->bytes % 16 != 0) return fail(ctx, NUQ_INVALID_SHAPE, "cache bytes must be 16-byte aligned");
+    view->bytes = (uint8_t *)c->bytes;
+    view->pages = (uint32_t)c->pages;
+    view->kv_heads = c->kv_heads;
+    view->tiles_log2 = (uint32_t)__builtin_ctz(c->page_tokens / 16);
+    return NUQ_OK;
+}
+
+// Rows of heads that a kernel reads or writes 16 bytes at a time.
+int check_head_rows(nuq_context *ctx, const char *what, const void *p, uint32_t dtype, uint64_t stride, uint64_t width,
+                    uint64_t rows) {
+    if (!p) return fail(ctx, NUQ_INVALID_ARGUMENT, "null %s", what);
+    const uint64_t elem = dtype == NUQ_F16 ? 2 : 4;
+    if (stride < width && rows > 1) return fail(ctx, NUQ_INVALID_SHAPE, "%s: rows of %llu overlap", what,
+                                                (unsigned long long)stride);
+    if (stride > (1ull << 40)) return fail(ctx, NUQ_INVALID_SHAPE, "%s: stride out of range", what);
+    if ((uintptr_t)p % 16 != 0 || (rows > 1 && stride * elem % 16 != 0))
+        return fail(ctx, NUQ_INVALID_SHAPE, "%s must be 16-byte aligned rows", what);
+    return NUQ_OK;
+}
+
+// What the write and the read share.
+int check_slots(nuq_context *ctx, const nuq_cache *cache, const void *k, const void *v, uint32_t dtype,
+                uint64_t k_stride, uint64_t v_stride, const int64_t *slots, uint64_t tokens, nuq::CacheView *view) {
+    int e = check_cache(ctx, cache, view);
+    if (e) return e;
+    if (dtype != NUQ_F32 && dtype != NUQ_F16) return fail(ctx, NUQ_INVALID_ARGUMENT, "unknown dtype");
+    if (tokens > (1ull << 26)) return fail(ctx, NUQ_INVALID_SHAPE, "more than 2^26 tokens");
+    if (tokens == 0) return NUQ_OK;
+    const uint64_t width = (uint64_t)cache->kv_heads * cache->head_dim;
+    if ((e = check_head_rows(ctx, "k", k, dtype, k_stride, width, tokens))) return e;
+    if ((e = check_head_rows(ctx, "v", v, dtype, v_stride, width, tokens))) return e;
+    if (!slots || (uintptr_t)slots % 8 != 0) return fail(ctx, NUQ_INVALID_ARGUMENT, "null or misaligned slots");
+    return NUQ_OK;
 }
 
 }  // namespace
@@ -746,6 +804,91 @@ int nuq_topk(nuq_context *ctx, const float *logits, uint64_t count, uint32_t k, 
                      nuq::launch_topk(ctx->stream, logits, (uint32_t)count, k, temperature, ctx->topk_keys,
                                       out->values, out->indices, out->sums, out->flags),
                      "top-k launch");
+}
+
+int nuq_cache_bytes(const nuq_cache *cache, uint64_t *bytes) {
+    if (!cache || !bytes) return NUQ_INVALID_ARGUMENT;
+    const uint64_t n = cache_bytes(cache);
+    if (n == 0) return NUQ_INVALID_SHAPE;
+    *bytes = n;
+    return NUQ_OK;
+}
+
+int nuq_cache_write(nuq_context *ctx, const nuq_cache *cache, const void *k, const void *v, uint32_t dtype,
+                    uint64_t k_stride, uint64_t v_stride, const int64_t *slots, uint64_t tokens) {
+    if (!ctx) return NUQ_INVALID_ARGUMENT;
+    nuq::CacheView view;
+    const int e = check_slots(ctx, cache, k, v, dtype, k_stride, v_stride, slots, tokens, &view);
+    if (e || tokens == 0) return e;
+    return hip_check(ctx,
+                     nuq::launch_cache_write(ctx->stream, view, cache->bits, cache->head_dim, dtype == NUQ_F16, k, v,
+                                             k_stride, v_stride, slots, tokens),
+                     "cache write launch");
+}
+
+int nuq_cache_read(nuq_context *ctx, const nuq_cache *cache, const int64_t *slots, uint64_t tokens, uint32_t dtype,
+                   void *k, void *v, uint64_t k_stride, uint64_t v_stride) {
+    if (!ctx) return NUQ_INVALID_ARGUMENT;
+    nuq::CacheView view;
+    const int e = check_slots(ctx, cache, k, v, dtype, k_stride, v_stride, slots, tokens, &view);
+    if (e || tokens == 0) return e;
+    return hip_check(ctx,
+                     nuq::launch_cache_read(ctx->stream, view, cache->bits, cache->head_dim, dtype == NUQ_F16, slots,
+                                            tokens, k, v, k_stride, v_stride),
+                     "cache read launch");
+}
+
+int nuq_cache_attention(nuq_context *ctx, const nuq_cache *cache, const nuq_attention *args) {
+    if (!ctx) return NUQ_INVALID_ARGUMENT;
+    nuq::CacheView view;
+    int e = check_cache(ctx, cache, &view);
+    if (e) return e;
+    if (!args) return fail(ctx, NUQ_INVALID_ARGUMENT, "null attention arguments");
+    const nuq_attention &n = *args;
+    if (n.dtype != NUQ_F32 && n.dtype != NUQ_F16) return fail(ctx, NUQ_INVALID_ARGUMENT, "unknown dtype");
+    if (n.q_heads == 0 || n.q_heads % cache->kv_heads != 0 || n.q_heads > 65535)
+        return fail(ctx, NUQ_INVALID_SHAPE, "%u query heads over %u KV heads", n.q_heads, cache->kv_heads);
+    if (!std::isfinite(n.scale) || n.scale <= 0)
+        return fail(ctx, NUQ_INVALID_SHAPE, "the scale must be finite and positive");
+    const uint64_t width = (uint64_t)n.q_heads * cache->head_dim;
+    // rows and positions are ints in the kernels
+    if (n.rows > 0x7fffffffull / n.q_heads || n.batch > 0x7fffffffu || n.max_tokens > n.rows)
+        return fail(ctx, NUQ_INVALID_SHAPE, "rows, batch or max_tokens out of range");
+    if (n.rows == 0 || n.batch == 0 || n.max_tokens == 0) return NUQ_OK;
+    if (!n.starts && n.rows != (uint64_t)n.batch * n.max_tokens)
+        return fail(ctx, NUQ_INVALID_SHAPE, "%llu rows are not %u sequences of %u", (unsigned long long)n.rows, n.batch,
+                    n.max_tokens);
+    if (n.table_width == 0 || n.table_width > (1ull << 30) / cache->page_tokens || n.table_stride > (1ull << 30) ||
+        (n.table_stride < n.table_width && n.batch > 1))
+        return fail(ctx, NUQ_INVALID_SHAPE, "page table of width %llu, stride %llu", (unsigned long long)n.table_width,
+                    (unsigned long long)n.table_stride);
+    if ((e = check_head_rows(ctx, "q", n.q, n.dtype, n.q_stride, width, n.rows))) return e;
+    if ((e = check_head_rows(ctx, "out", n.out, n.dtype, n.out_stride, width, n.rows))) return e;
+    if (!n.page_table || !n.lengths) return fail(ctx, NUQ_INVALID_ARGUMENT, "null page table or lengths");
+    if ((uintptr_t)n.page_table % 4 || (uintptr_t)n.lengths % 4 || (uintptr_t)n.starts % 4)
+        return fail(ctx, NUQ_INVALID_SHAPE, "page table, lengths and starts must be 4-byte aligned");
+    nuq::AttentionArgs a{};
+    a.q = n.q, a.out = n.out, a.q_stride = n.q_stride, a.out_stride = n.out_stride;
+    a.table = n.page_table, a.lengths = n.lengths, a.starts = n.starts, a.table_stride = n.table_stride;
+    a.rows = (uint32_t)n.rows, a.batch = n.batch, a.max_tokens = n.max_tokens, a.group = n.q_heads / cache->kv_heads;
+    a.capacity = (uint32_t)(n.table_width * cache->page_tokens);
+    a.window = n.window >= a.capacity ? 0 : n.window;
+    a.scale = n.scale * 1.44269504088896340736f;
+    const uint64_t longest = n.max_length ? std::min<uint64_t>(n.max_length, a.capacity) : a.capacity;
+    const uint32_t f32 = n.dtype == NUQ_F32;
+    const auto plan_with = [&](uint64_t floats) {
+        nuq::plan_attention(cache->bits, cache->head_dim, cache->kv_heads, f32, longest, n.q_heads, floats, &a);
+    };
+    plan_with(UINT64_MAX);
+    // without the workspace it wants (a capture, no memory): fewer splits
+    if (!ensure_workspace(ctx, a.floats)) plan_with((uint64_t)ctx->split.tiles * 256 * 256);
+    if ((uint64_t)cache->kv_heads * a.splits * a.blocks * a.batch > 0x00ffffffull ||
+        (uint64_t)a.batch * a.max_tokens * n.q_heads > 0x03ffffffull)
+        return fail(ctx, NUQ_INVALID_SHAPE, "too many query rows for one call");
+    return hip_check(ctx,
+                     nuq::launch_attention(ctx->stream, view, cache->bits, cache->head_dim, f32, n.q_heads, a,
+                                           ctx->split.work),
+                     "attention launch");
 }
 
 // The tensor-data section of a GGUF file goes to the device unchanged

@@ -1,0 +1,36 @@
+// Launchers of the attention over the quantised cache (attention.hip).
+#pragma once
+
+#include <type_traits>
+
+#include "cache.h"
+
+namespace nuq {
+
+struct AttentionArgs {
+    const void *q;
+    void *out;
+    uint64_t q_stride, out_stride;  // elements from a query row to the next
+    const int32_t *table;           // [batch][table_stride] page numbers
+    const int32_t *lengths;         // [batch] tokens held, the new ones among them
+    const int32_t *starts;          // [batch + 1] first query row of each sequence; null: max_tokens each
+    uint64_t table_stride;
+    uint32_t rows;        // query rows in all
+    uint32_t batch, max_tokens, group;
+    uint32_t capacity;    // tokens a row of the table can name
+    uint32_t window;      // 0: none
+    float scale;          // of the scores, log2(e) among it
+    // the plan
+    uint32_t row_tiles, blocks, splits;
+    uint64_t floats;      // of workspace
+    float *partial_o, *partial_ml;
+};
+
+// Fills in the plan of a call: row tiles of 16, blocks of them, splits of the
+// long axis with at most `max_floats` of workspace.
+void plan_attention(uint32_t bits, uint32_t head_dim, uint32_t kv_heads, uint32_t f32, uint64_t max_length,
+                    uint32_t heads, uint64_t max_floats, AttentionArgs *a);
+hipError_t launch_attention(hipStream_t s, const CacheView &c, uint32_t bits, uint32_t head_dim, uint32_t f32,
+                            uint32_t heads, AttentionArgs a, float *work);
+
+}  // namespace nuq

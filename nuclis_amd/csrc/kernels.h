@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "cache.h"
 #include "panel.h"
 
 namespace nuq {
@@ -82,6 +83,16 @@ hipError_t launch_penalize(hipStream_t s, float *logits, uint32_t count, const u
                            float presence);
 hipError_t launch_topk(hipStream_t s, const float *logits, uint32_t count, uint32_t k, float temperature,
                        uint64_t *scratch, float *values, uint32_t *indices, float *sums, uint32_t *flags);
+
+// The quantised cache (cache.hip): tokens into their slots and back.
+uint64_t cache_tile_bytes(uint32_t bits, uint32_t head_dim);
+hipError_t launch_cache_write(hipStream_t s, const CacheView &c, uint32_t bits, uint32_t head_dim, uint32_t f16,
+                              const void *k, const void *v, uint64_t k_stride, uint64_t v_stride, const int64_t *slots,
+                              uint64_t tokens);
+hipError_t launch_cache_read(hipStream_t s, const CacheView &c, uint32_t bits, uint32_t head_dim, uint32_t f16,
+                             const int64_t *slots, uint64_t tokens, void *k, void *v, uint64_t k_stride,
+                             uint64_t v_stride);
+
 // How a product runs on the tiles (plan_tile): the route, its panel plan (and
 // that of a shorter last chunk), the tokens served per chunk, the floats of the
 // f16 copy of F32 activations and the workspace it uses in all (split
