@@ -281,6 +281,21 @@ typedef struct nuq_attention {
 } nuq_attention;
 int nuq_cache_attention(nuq_context *ctx, const nuq_cache *cache, const nuq_attention *args);
 
+/* Log probabilities of given tokens: for each of `rows` rows of `count` logits
+ * (F32 or F16, `stride` elements apart) log softmax at targets[row], the entropy
+ * of the softmax (natural logarithms), and the `top` most probable tokens by (logit
+ * descending, id ascending) with their log probabilities. All but the logits'
+ * dtype is F32 / 32-bit, in device memory: logprobs and entropy [rows], top_ids and
+ * top_logprobs [rows][top] (not read where top is 0). A logit of -inf is a token
+ * of probability zero; a row of them alone gives -inf and entropy 0. A NaN or
+ * +inf makes its row's results NaN (NaN never enters the list; ids past the
+ * numbers there are, 0xffffffff with -inf). A target outside [0, count) gives
+ * NaN. Beyond Backend.topk: the reference's sampler has no scoring of given tokens. */
+enum { NUQ_LOGPROBS_MAX_TOP = 32 };
+int nuq_logprobs(nuq_context *ctx, const void *logits, uint32_t dtype, uint64_t rows, uint64_t count, uint64_t stride,
+                 const int32_t *targets, uint32_t top, float *logprobs, float *entropy, uint32_t *top_ids,
+                 float *top_logprobs);
+
 /* Weight preparation on the host (not part of the reference's backend):
  * quantize `rows` F32 rows of `columns` into GGUF rows in dst (host memory,
  * dst_len = rows * row bytes). Q8_0 is quant/encode.zig:17-36 exactly; the

@@ -81,6 +81,8 @@ class _TopKBuffers(ctypes.Structure):
                 ("flags", ctypes.c_void_p)]
 
 
+LOGPROBS_MAX_TOP = 32  # NUQ_LOGPROBS_MAX_TOP (include/nuq.h)
+
 # Backend.topk limits (backends/metal/ops/sampling.zig:15-22)
 TOPK_CAPACITY, TOPK_PARTIALS, TOPK_MAX_COUNT = 256, 64, 262144
 
@@ -126,6 +128,7 @@ EXPORTS = [
     "nuq_matmul_kernel", "nuq_matvec_segments", "nuq_argmax", "nuq_quantize_rows", "nuq_dequant_rows", "nuq_gemv",
     "nuq_gemm", "nuq_topk", "nuq_penalize", "nuq_reserve_workspace", "nuq_workspace_bytes",
     "nuq_matvec_segments_noalloc", "nuq_cache_bytes", "nuq_cache_write", "nuq_cache_read", "nuq_cache_attention",
+    "nuq_logprobs",
 ]
 
 
@@ -171,6 +174,7 @@ def lib() -> ctypes.CDLL:
         L.nuq_cache_write.argtypes = [vp, cp, vp, vp, u32, u64, u64, vp, u64]
         L.nuq_cache_read.argtypes = [vp, cp, vp, u64, u32, vp, vp, u64, u64]
         L.nuq_cache_attention.argtypes = [vp, cp, ctypes.POINTER(_Attention)]
+        L.nuq_logprobs.argtypes = [vp, vp, u32, u64, u64, u64, vp, u32, vp, vp, vp, vp]
         _lib = L
     return _lib
 
@@ -388,7 +392,7 @@ class Backend:
 
     # -- the quantised cache and the attention over it ------------------------
     def _index(self, t, dtype, name: str):
-        """A contiguous index tensor's address."""
+        """The address of a contiguous tensor of this dtype."""
         if t.dtype is not dtype:
             raise InvalidArgument(f"{name} must be {dtype}, not {t.dtype}")
         if not t.is_contiguous():
@@ -460,6 +464,34 @@ class Backend:
                           None if starts is None else self._index(starts, int32, "starts"), batch, max_tokens,
                           max_length, cache.head_dim ** -0.5 if scale is None else scale, window)
         self._call(lib().nuq_cache_attention, ctypes.byref(cache._c), ctypes.byref(args))
+
+    def logprobs(self, logits, targets, logprobs, entropy, top_ids=None, top_logprobs=None) -> None:
+        """Log probabilities of given tokens (nuq_logprobs, include/nuq.h):
+        logits [rows][count] (F32 or F16, rows may be strided), targets int32
+        [rows]; logprobs and entropy F32 [rows]; top_ids int32 and top_logprobs F32
+        [rows][top], the most probable tokens (both or neither)."""
+        torch = self._torch
+        if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+            raise InvalidShape(f"InvalidShape: logits {tuple(logits.shape)} are not contiguous rows")
+        if logits.dtype is not torch.float32 and logits.dtype is not torch.float16:
+            raise InvalidArgument(f"logits are {logits.dtype}, not float32 or float16")
+        rows, count = logits.shape
+        if targets.numel() != rows or logprobs.numel() != rows or entropy.numel() != rows:
+            raise InvalidShape(f"InvalidShape: targets or results are not of {rows} rows")
+        if (top_ids is None) != (top_logprobs is None):
+            raise InvalidArgument("top_ids and top_logprobs come together")
+        top, ids, tops = 0, None, None
+        if top_ids is not None:
+            if top_ids.dim() != 2 or top_ids.shape[0] != rows or top_ids.shape != top_logprobs.shape:
+                raise InvalidShape(f"InvalidShape: top_ids {tuple(top_ids.shape)} and top_logprobs "
+                                   f"{tuple(top_logprobs.shape)} for {rows} rows")
+            top = top_ids.shape[1]
+            ids = self._index(top_ids, torch.int32, "top_ids")
+            tops = self._index(top_logprobs, torch.float32, "top_logprobs")
+        self._call(lib().nuq_logprobs, logits.data_ptr(), F16 if logits.dtype is torch.float16 else F32, rows, count,
+                   logits.stride(0), self._index(targets, torch.int32, "targets"), top,
+                   self._index(logprobs, torch.float32, "logprobs"), self._index(entropy, torch.float32, "entropy"),
+                   ids, tops)
 
     def argmax(self, logits) -> int:
         idx = ctypes.c_uint32(0)

@@ -891,6 +891,31 @@ int nuq_cache_attention(nuq_context *ctx, const nuq_cache *cache, const nuq_atte
                      "attention launch");
 }
 
+int nuq_logprobs(nuq_context *ctx, const void *logits, uint32_t dtype, uint64_t rows, uint64_t count, uint64_t stride,
+                 const int32_t *targets, uint32_t top, float *logprobs, float *entropy, uint32_t *top_ids,
+                 float *top_logprobs) {
+    if (!ctx) return NUQ_INVALID_ARGUMENT;
+    if (dtype != NUQ_F32 && dtype != NUQ_F16) return fail(ctx, NUQ_INVALID_ARGUMENT, "unknown logit dtype");
+    if (count == 0 || count > (1ull << 30) || rows > (1ull << 23) || stride > (1ull << 40) ||
+        (stride < count && rows > 1))
+        return fail(ctx, NUQ_INVALID_SHAPE, "%llu rows of %llu logits, stride %llu", (unsigned long long)rows,
+                    (unsigned long long)count, (unsigned long long)stride);
+    if (top > NUQ_LOGPROBS_MAX_TOP || top > count)
+        return fail(ctx, NUQ_INVALID_SHAPE, "top %u of %llu logits is out of range", top, (unsigned long long)count);
+    if (rows == 0) return NUQ_OK;
+    if (!logits || !targets || !logprobs || !entropy || (top && (!top_ids || !top_logprobs)))
+        return fail(ctx, NUQ_INVALID_ARGUMENT, "null logits, targets or results");
+    if ((uintptr_t)logits % (dtype == NUQ_F16 ? 2 : 4) ||
+        ((uintptr_t)targets | (uintptr_t)logprobs | (uintptr_t)entropy | (uintptr_t)top_ids | (uintptr_t)top_logprobs) % 4)
+        return fail(ctx, NUQ_INVALID_SHAPE, "misaligned logits, targets or results");
+    (void)ensure_workspace(ctx, nuq::logprobs_floats((uint32_t)rows, (uint32_t)count, top));
+    return hip_check(ctx,
+                     nuq::launch_logprobs(ctx->stream, logits, dtype == NUQ_F16, (uint32_t)rows, (uint32_t)count, stride,
+                                          targets, top, logprobs, entropy, top_ids, top_logprobs, ctx->split.work,
+                                          (uint64_t)ctx->split.tiles * 256 * 256),
+                     "log probabilities launch");
+}
+
 // The tensor-data section of a GGUF file goes to the device unchanged
 // (tensors keep their offsets). Host threads copy the mapping into one of
 // two pinned staging buffers while the DMA engine drains the other, so the

@@ -84,6 +84,14 @@ hipError_t launch_penalize(hipStream_t s, float *logits, uint32_t count, const u
 hipError_t launch_topk(hipStream_t s, const float *logits, uint32_t count, uint32_t k, float temperature,
                        uint64_t *scratch, float *values, uint32_t *indices, float *sums, uint32_t *flags);
 
+// Log probabilities of rows of logits (logprobs.hip); `floats` of workspace,
+// without which a row is not split over workgroups.
+constexpr uint32_t LOGPROBS_MAX_TOP = 32;
+uint64_t logprobs_floats(uint32_t rows, uint32_t count, uint32_t top);
+hipError_t launch_logprobs(hipStream_t s, const void *logits, uint32_t f16, uint32_t rows, uint32_t count,
+                           uint64_t stride, const int32_t *targets, uint32_t top, float *logprobs, float *entropy,
+                           uint32_t *ids, float *tops, float *work, uint64_t floats);
+
 // The quantised cache (cache.hip): tokens into their slots and back.
 uint64_t cache_tile_bytes(uint32_t bits, uint32_t head_dim);
 hipError_t launch_cache_write(hipStream_t s, const CacheView &c, uint32_t bits, uint32_t head_dim, uint32_t f16,
