@@ -258,8 +258,8 @@ class KVCache:
         elif not bytes.is_contiguous():
             raise InvalidShape("InvalidShape: the cache's bytes are not contiguous")
         self.bytes = bytes
-        self._c = _Cache(bits, page_tokens, kv_heads, head_dim, pages, bytes.data_ptr(),
-                         bytes.numel() * bytes.element_size())
+        self._ref = ctypes.byref(_Cache(bits, page_tokens, kv_heads, head_dim, pages, bytes.data_ptr(),
+                                        bytes.numel() * bytes.element_size()))
 
 
 def _ptr(t) -> int | None:
@@ -274,6 +274,10 @@ class Backend:
 
         self._torch = torch
         self.device = device
+        self._float_codes = {torch.float32: F32, torch.float16: F16}
+        # the current stream's handle without a Stream object around it (1 us a call)
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        self._raw_stream = raw or (lambda d: torch.cuda.current_stream(d).cuda_stream)
         err = ctypes.create_string_buffer(512)
         with torch.cuda.device(device):
             self._h = lib().nuq_create(device, err, len(err))
@@ -293,7 +297,7 @@ class Backend:
 
     # -- plumbing -----------------------------------------------------------
     def _call(self, fn, *args) -> None:
-        stream = self._torch.cuda.current_stream(self.device).cuda_stream
+        stream = self._raw_stream(self.device)
         # a change of stream makes the new one wait for the old one's work
         # (the context's workspace is shared by its calls)
         code = lib().nuq_set_stream(self._h, stream)
@@ -391,6 +395,8 @@ class Backend:
                     values.cpu().tolist()[:k], total, not bool(flags.cpu().any()))
 
     # -- the quantised cache and the attention over it ------------------------
+    # (shapes, strides and dtypes are asked for once each: a decode step makes
+    # these calls for every layer, and each question to a tensor is 0.1 us)
     def _index(self, t, dtype, name: str):
         """The address of a contiguous tensor of this dtype."""
         if t.dtype is not dtype:
@@ -399,40 +405,41 @@ class Backend:
             raise InvalidShape(f"InvalidShape: {name} is not contiguous")
         return t.data_ptr()
 
-    def _heads(self, t, heads: int, head_dim: int, name: str) -> int:
-        """Checks [rows][heads][head_dim] with contiguous rows; the dtype's code."""
-        if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != head_dim:
-            raise InvalidShape(f"InvalidShape: {name} is {tuple(t.shape)}, not [rows][{heads}][{head_dim}]")
-        stride = t.stride()
-        if stride[2] != 1 or (heads > 1 and stride[1] != head_dim):
+    def _heads(self, t, head_dim: int, name: str):
+        """Checks [rows][heads][head_dim] with contiguous rows: (rows, heads, elements from a row to the
+        next, the dtype's code)."""
+        shape, stride = t.shape, t.stride()
+        if len(shape) != 3 or shape[2] != head_dim:
+            raise InvalidShape(f"InvalidShape: {name} is {tuple(shape)}, not [rows][heads][{head_dim}]")
+        rows, heads, _ = shape
+        if stride[2] != 1 or (stride[1] != head_dim and heads > 1):
             raise InvalidShape(f"InvalidShape: {name}'s rows are not contiguous")
-        if t.dtype is self._torch.float32:
-            return F32
-        if t.dtype is self._torch.float16:
-            return F16
-        raise InvalidArgument(f"{name} is {t.dtype}, not float32 or float16")
+        code = self._float_codes.get(t.dtype)
+        if code is None:
+            raise InvalidArgument(f"{name} is {t.dtype}, not float32 or float16")
+        return rows, heads, stride[0], code
 
     def _slots(self, cache: KVCache, k, v, slots):
-        dtype = self._heads(k, cache.kv_heads, cache.head_dim, "k")
-        if self._heads(v, cache.kv_heads, cache.head_dim, "v") != dtype:
+        tokens, heads, k_stride, code = self._heads(k, cache.head_dim, "k")
+        v_tokens, v_heads, v_stride, v_code = self._heads(v, cache.head_dim, "v")
+        if v_code != code:
             raise InvalidArgument("k and v differ in dtype")
-        tokens = slots.numel()
-        if k.shape[0] != tokens or v.shape[0] != tokens:
-            raise InvalidShape(f"InvalidShape: {tokens} slots for {k.shape[0]} keys and {v.shape[0]} values")
-        return dtype, tokens, self._index(slots, self._torch.int64, "slots")
+        if heads != cache.kv_heads or v_heads != heads:
+            raise InvalidShape(f"InvalidShape: {heads} and {v_heads} heads for a cache of {cache.kv_heads}")
+        if slots.numel() != tokens or v_tokens != tokens:
+            raise InvalidShape(f"InvalidShape: {slots.numel()} slots for {tokens} keys and {v_tokens} values")
+        return code, tokens, k_stride, v_stride, self._index(slots, self._torch.int64, "slots")
 
     def cache_write(self, cache: KVCache, k, v, slots) -> None:
         """Quantises tokens' keys and values [tokens][kv_heads][head_dim] (F32
         or F16; rows may be strided) into their slots (int64; -1 skips)."""
-        dtype, tokens, at = self._slots(cache, k, v, slots)
-        self._call(lib().nuq_cache_write, ctypes.byref(cache._c), k.data_ptr(), v.data_ptr(), dtype, k.stride(0),
-                   v.stride(0), at, tokens)
+        code, tokens, k_stride, v_stride, at = self._slots(cache, k, v, slots)
+        self._call(_lib.nuq_cache_write, cache._ref, k.data_ptr(), v.data_ptr(), code, k_stride, v_stride, at, tokens)
 
     def cache_read(self, cache: KVCache, slots, k, v) -> None:
         """Reads slots back into k and v (F32 or F16, both exact)."""
-        dtype, tokens, at = self._slots(cache, k, v, slots)
-        self._call(lib().nuq_cache_read, ctypes.byref(cache._c), at, tokens, dtype, k.data_ptr(), v.data_ptr(),
-                   k.stride(0), v.stride(0))
+        code, tokens, k_stride, v_stride, at = self._slots(cache, k, v, slots)
+        self._call(_lib.nuq_cache_read, cache._ref, at, tokens, code, k.data_ptr(), v.data_ptr(), k_stride, v_stride)
 
     def cache_attention(self, cache: KVCache, q, output, page_table, lengths, starts=None, scale: float | None = None,
                         window: int = 0, max_tokens: int | None = None, max_length: int = 0) -> None:
@@ -442,28 +449,31 @@ class Backend:
         int32 [batch + 1] where the sequences bring different counts of rows.
         `scale` is head_dim ** -0.5 by default; `max_tokens` (a bound on a
         sequence's rows) and `max_length` (on its tokens) size the launch."""
-        if q.dim() != 3:
-            raise InvalidShape(f"InvalidShape: q is {tuple(q.shape)}, not [rows][q_heads][head_dim]")
-        rows, heads = q.shape[0], q.shape[1]
-        dtype = self._heads(q, heads, cache.head_dim, "q")
-        if self._heads(output, heads, cache.head_dim, "output") != dtype or output.shape[0] != rows:
+        rows, heads, q_stride, code = self._heads(q, cache.head_dim, "q")
+        out_rows, out_heads, out_stride, out_code = self._heads(output, cache.head_dim, "output")
+        if out_rows != rows or out_heads != heads or out_code != code:
             raise InvalidShape("InvalidShape: the output is not of q's shape and dtype")
         int32 = self._torch.int32
         batch = lengths.numel()
-        if page_table.dim() != 2 or page_table.shape[0] != batch:
-            raise InvalidShape(f"InvalidShape: page table {tuple(page_table.shape)} for {batch} sequences")
-        if page_table.dtype is not int32 or page_table.stride(1) != 1:
+        table, table_stride = page_table.shape, page_table.stride()
+        if len(table) != 2 or table[0] != batch:
+            raise InvalidShape(f"InvalidShape: page table {tuple(table)} for {batch} sequences")
+        if page_table.dtype is not int32 or table_stride[1] != 1:
             raise InvalidArgument("the page table is not int32 with contiguous rows")
-        if starts is not None and starts.numel() != batch + 1:
-            raise InvalidShape(f"InvalidShape: {starts.numel()} starts for {batch} sequences")
+        first = None
+        if starts is not None:
+            if starts.numel() != batch + 1:
+                raise InvalidShape(f"InvalidShape: {starts.numel()} starts for {batch} sequences")
+            first = self._index(starts, int32, "starts")
         if max_tokens is None:
             max_tokens = rows if starts is not None else rows // max(batch, 1)
-        args = _Attention(q.data_ptr(), output.data_ptr(), dtype, heads, q.stride(0), output.stride(0), rows,
-                          page_table.data_ptr(), page_table.stride(0), page_table.shape[1],
-                          self._index(lengths, int32, "lengths"),
-                          None if starts is None else self._index(starts, int32, "starts"), batch, max_tokens,
-                          max_length, cache.head_dim ** -0.5 if scale is None else scale, window)
-        self._call(lib().nuq_cache_attention, ctypes.byref(cache._c), ctypes.byref(args))
+        if not (0 <= window < 1 << 32 and 0 <= max_tokens < 1 << 32 and 0 <= max_length < 1 << 63):
+            raise InvalidShape(f"InvalidShape: window {window}, max_tokens {max_tokens}, max_length {max_length}")
+        args = _Attention(q.data_ptr(), output.data_ptr(), code, heads, q_stride, out_stride, rows,
+                          page_table.data_ptr(), table_stride[0], table[1], self._index(lengths, int32, "lengths"),
+                          first, batch, max_tokens, max_length, cache.head_dim ** -0.5 if scale is None else scale,
+                          window)
+        self._call(_lib.nuq_cache_attention, cache._ref, ctypes.byref(args))
 
     def logprobs(self, logits, targets, logprobs, entropy, top_ids=None, top_logprobs=None) -> None:
         """Log probabilities of given tokens (nuq_logprobs, include/nuq.h):
@@ -471,27 +481,29 @@ class Backend:
         [rows]; logprobs and entropy F32 [rows]; top_ids int32 and top_logprobs F32
         [rows][top], the most probable tokens (both or neither)."""
         torch = self._torch
-        if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
-            raise InvalidShape(f"InvalidShape: logits {tuple(logits.shape)} are not contiguous rows")
-        if logits.dtype is not torch.float32 and logits.dtype is not torch.float16:
+        shape, stride = logits.shape, logits.stride()
+        if len(shape) != 2 or (stride[1] != 1 and shape[1] > 1):
+            raise InvalidShape(f"InvalidShape: logits {tuple(shape)} are not contiguous rows")
+        code = self._float_codes.get(logits.dtype)
+        if code is None:
             raise InvalidArgument(f"logits are {logits.dtype}, not float32 or float16")
-        rows, count = logits.shape
+        rows, count = shape
         if targets.numel() != rows or logprobs.numel() != rows or entropy.numel() != rows:
             raise InvalidShape(f"InvalidShape: targets or results are not of {rows} rows")
         if (top_ids is None) != (top_logprobs is None):
             raise InvalidArgument("top_ids and top_logprobs come together")
         top, ids, tops = 0, None, None
         if top_ids is not None:
-            if top_ids.dim() != 2 or top_ids.shape[0] != rows or top_ids.shape != top_logprobs.shape:
-                raise InvalidShape(f"InvalidShape: top_ids {tuple(top_ids.shape)} and top_logprobs "
+            tops_shape = top_ids.shape
+            if len(tops_shape) != 2 or tops_shape[0] != rows or tops_shape != top_logprobs.shape:
+                raise InvalidShape(f"InvalidShape: top_ids {tuple(tops_shape)} and top_logprobs "
                                    f"{tuple(top_logprobs.shape)} for {rows} rows")
-            top = top_ids.shape[1]
+            top = tops_shape[1]
             ids = self._index(top_ids, torch.int32, "top_ids")
             tops = self._index(top_logprobs, torch.float32, "top_logprobs")
-        self._call(lib().nuq_logprobs, logits.data_ptr(), F16 if logits.dtype is torch.float16 else F32, rows, count,
-                   logits.stride(0), self._index(targets, torch.int32, "targets"), top,
-                   self._index(logprobs, torch.float32, "logprobs"), self._index(entropy, torch.float32, "entropy"),
-                   ids, tops)
+        self._call(_lib.nuq_logprobs, logits.data_ptr(), code, rows, count, stride[0],
+                   self._index(targets, torch.int32, "targets"), top, self._index(logprobs, torch.float32, "logprobs"),
+                   self._index(entropy, torch.float32, "entropy"), ids, tops)
 
     def argmax(self, logits) -> int:
         idx = ctypes.c_uint32(0)

@@ -46,7 +46,7 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 constexpr float LOWEST = -3.402823466e38f;  // a running maximum before any token
 constexpr float RAISE = 7.0f;   // P is 2^RAISE at the reference
 constexpr float SLACK = 8.0f;   // how far (log2) a score may pass the reference
-constexpr int WAVES = 4, STEP = 32;
+constexpr int WAVES = 4, STEP = 32, MAX_SPLITS = 64;
 
 __device__ __forceinline__ half2v as_half2(uint32_t u) { return __builtin_bit_cast(half2v, u); }
 __device__ __forceinline__ uint32_t as_u32(half2v h) { return __builtin_bit_cast(uint32_t, h); }
@@ -109,6 +109,14 @@ __device__ __forceinline__ void decode_v(const uint32_t *c, int pair, half2v d, 
         out[2] = as_u32(as_half2(__builtin_amdgcn_perm(e, a, 0x0c060c02u) | 0x64006400u) * d + b);
         out[3] = as_u32(as_half2(__builtin_amdgcn_perm(e, a, 0x0c070c03u) | 0x64006400u) * d + b);
     }
+}
+
+__device__ __forceinline__ void store4(float *to, const float4 &x, float by) {
+    *(float4 *)to = make_float4(x.x * by, x.y * by, x.z * by, x.w * by);
+}
+__device__ __forceinline__ void store4(_Float16 *to, const float4 &x, float by) {
+    const half2v lo = {(_Float16)(x.x * by), (_Float16)(x.y * by)}, hi = {(_Float16)(x.z * by), (_Float16)(x.w * by)};
+    *(uint2 *)to = make_uint2(as_u32(lo), as_u32(hi));
 }
 
 template <int BYTES> __device__ __forceinline__ void load_words(uint32_t *to, const uint8_t *p) {
@@ -467,51 +475,65 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_rows_kernel(CacheView
             if (partial) {
                 *(float4 *)(partial + at) = x;
             } else {
-                T *to = (T *)a.out + out_row * a.out_stride + out_head * D + at;
-                if constexpr (F32) {
-                    *(float4 *)to = make_float4(x.x * inverse, x.y * inverse, x.z * inverse, x.w * inverse);
-                } else {
-                    const half2v lo = {(_Float16)(x.x * inverse), (_Float16)(x.y * inverse)};
-                    const half2v hi = {(_Float16)(x.z * inverse), (_Float16)(x.w * inverse)};
-                    *(uint2 *)to = make_uint2(as_u32(lo), as_u32(hi));
-                }
+                store4((T *)a.out + out_row * a.out_stride + out_head * D + at, x, inverse);
             }
         }
     }
 }
 
-// Joins the splits of one (sequence, token, head) a wave. A split without a
-// token has sum 0 and no output: it is not read.
+// Joins the splits of one (sequence, token, head) a workgroup: the first wave
+// turns the splits' maxima into weights, then D / 4 threads take a split, 1024 / D
+// splits at a time. A split without a token has sum 0 and no output: it is not
+// read. (One wave walking 64 splits in order took 29 us after 32768 tokens,
+// one round of memory latency a split; this takes 3.9.)
 template <int D, bool F32>
 __global__ void __launch_bounds__(256) attention_join_kernel(AttentionArgs a, uint32_t heads) {
     using T = std::conditional_t<F32, float, _Float16>;
-    constexpr int EACH = D / 64;
-    const uint64_t id = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = (int)threadIdx.x & 63;
-    const uint32_t head = (uint32_t)(id % heads), token = (uint32_t)(id / heads % a.max_tokens);
-    const uint64_t b = id / heads / a.max_tokens;
-    if (b >= a.batch) return;
+    constexpr int ACROSS = D / 4, SIDE = 256 / ACROSS;
+    __shared__ float weight[MAX_SPLITS], total;
+    __shared__ __align__(16) float part[SIDE][D];
+    const uint32_t head = blockIdx.x % heads, token = blockIdx.x / heads % a.max_tokens;
+    const uint32_t b = blockIdx.x / heads / a.max_tokens;
     int begin, tokens;
-    rows_of(a, (uint32_t)b, begin, tokens);
+    rows_of(a, b, begin, tokens);
     if ((int)token >= tokens) return;
     const uint64_t row = (uint64_t)begin + token, at = row * heads + head;
     const float *ml = a.partial_ml + 2 * at * a.splits;
-    float m = LOWEST;
-    for (uint32_t i = 0; i < a.splits; ++i) m = fmaxf(m, ml[2 * i]);
-    float x[EACH] = {}, whole = 0.0f;
-    for (uint32_t i = 0; i < a.splits; ++i) {
-        const float l = ml[2 * i + 1];
-        if (l == 0.0f) continue;
-        const float by = __builtin_amdgcn_exp2f(ml[2 * i] - m);
-        whole += by * l;
-        const float *p = a.partial_o + (at * a.splits + i) * D + lane * EACH;
+    const uint32_t tid = threadIdx.x;
+    if (tid < 64) {
+        float m = LOWEST, l = 0.0f;
+        if (tid < a.splits) m = ml[2 * tid], l = ml[2 * tid + 1];
+        float top = m;
 #pragma unroll
-        for (int e = 0; e < EACH; ++e) x[e] += by * p[e];
+        for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+        const float w = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+        float sum = l == 0.0f ? 0.0f : w * l;
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+        weight[tid] = l == 0.0f ? -1.0f : w;
+        if (tid == 0) total = sum;
     }
-    const float inverse = whole == 0.0f ? 0.0f : 1.0f / whole;
-    T *to = (T *)a.out + row * a.out_stride + head * D + lane * EACH;
+    __syncthreads();
+    const uint32_t side = tid / ACROSS, x4 = 4 * (tid % ACROSS);
+    const float *p = a.partial_o + at * a.splits * D + x4;
+    float4 x = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+    for (uint32_t i = side; i < a.splits; i += SIDE) {
+        const float w = weight[i];
+        float4 y = make_float4(0, 0, 0, 0);
+        if (w != -1.0f) y = *(const float4 *)(p + (uint64_t)i * D);
+        x.x += w * y.x, x.y += w * y.y, x.z += w * y.z, x.w += w * y.w;
+    }
+    *(float4 *)&part[side][x4] = x;
+    __syncthreads();
+    if (tid >= ACROSS) return;
 #pragma unroll
-    for (int e = 0; e < EACH; ++e) to[e] = (T)(x[e] * inverse);
+    for (int i = 1; i < SIDE; ++i) {
+        const float4 y = *(const float4 *)&part[i][x4];
+        x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+    }
+    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+    store4((T *)a.out + row * a.out_stride + head * D + x4, x, inverse);
 }
 
 template <int BITS, int D, int RT, bool F32>
@@ -556,7 +578,7 @@ void plan_attention(uint32_t bits, uint32_t head_dim, uint32_t kv_heads, uint32_
     // enough workgroups for two on every CU, each with at least one step a wave
     uint64_t splits = std::max<uint64_t>(1, std::min<uint64_t>((512 + groups - 1) / groups,
                                                               (reach + WAVES * STEP - 1) / (WAVES * STEP)));
-    splits = std::min<uint64_t>(splits, 64);
+    splits = std::min<uint64_t>(splits, MAX_SPLITS);
     const uint64_t each = (uint64_t)a->rows * heads * (head_dim + 2);
     if (splits > 1 && splits * each > max_floats) splits = std::max<uint64_t>(1, max_floats / each);
     a->splits = (uint32_t)splits;
@@ -571,7 +593,7 @@ hipError_t launch_attention(hipStream_t s, const CacheView &c, uint32_t bits, ui
     }
     const hipError_t e = f32 ? rows_dispatch<true>(s, c, bits, head_dim, a) : rows_dispatch<false>(s, c, bits, head_dim, a);
     if (e != hipSuccess || a.splits == 1) return e;
-    const uint32_t grid = (uint32_t)(((uint64_t)a.batch * a.max_tokens * heads + 3) / 4);
+    const uint32_t grid = a.batch * a.max_tokens * heads;
 #define NUQ_CASE(D)                                                                                  \
     if (head_dim == D) {                                                                             \
         if (f32) attention_join_kernel<D, true><<<grid, 256, 0, s>>>(a, heads);                      \

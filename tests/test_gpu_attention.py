@@ -287,6 +287,7 @@ def test_refusals_leave_the_output_untouched(backend):
         (dict(scale=0.0), nq.InvalidShape), (dict(scale=float("nan")), nq.InvalidShape),
         (dict(scale=-1.0), nq.InvalidShape), (dict(scale=float("inf")), nq.InvalidShape),
         (dict(max_tokens=3), nq.InvalidShape), (dict(max_tokens=5), nq.InvalidShape),
+        (dict(window=-1), nq.InvalidShape), (dict(max_tokens=-1), nq.InvalidShape), (dict(max_length=-1), nq.InvalidShape),
     ]
     for change, error in cases:
         args = dict(cache=c.cache, q=q, output=out, page_table=table, lengths=lengths, **{})
