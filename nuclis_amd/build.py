@@ -16,7 +16,8 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libnuq.so"
-SOURCES = ["api.hip", "gemv.hip", "gemv_int.hip", "gemm.hip", "panel_plan.hip", "sampling.hip", "cache.hip", "attention.hip", "logprobs.hip",
+SOURCES = ["api.hip", "gemv.hip", "gemv_int.hip", "gemm.hip", "panel_plan.hip", "sampling.hip", "cache.hip", "attention.hip", "attention_prompt.hip",
+           "logprobs.hip",
            "quantize.cpp", "gguf.cpp"]
 PANEL_ENCODINGS = [23, 13, 14, 12, 8]  # panel.hip is compiled once per encoding
 ARCH = "gfx950"

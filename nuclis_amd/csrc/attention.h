@@ -21,10 +21,18 @@ struct AttentionArgs {
     uint32_t window;      // 0: none
     float scale;          // of the scores, log2(e) among it
     // the plan
+    uint32_t prompt;      // the prompt kernel's call
     uint32_t row_tiles, blocks, splits;
     uint64_t floats;      // of workspace
     float *partial_o, *partial_ml;
 };
+
+// Row tiles of a wave of the prompt kernel (attention_prompt.hip).
+constexpr int prompt_row_tiles(int head_dim, bool f32) {
+    return head_dim == 64 ? (f32 ? 3 : 4) : head_dim == 128 ? (f32 ? 2 : 3) : (f32 ? 1 : 2);
+}
+hipError_t launch_attention_prompt(hipStream_t s, const CacheView &c, uint32_t bits, uint32_t d, uint32_t f32,
+                                   const AttentionArgs &a);
 
 // Fills in the plan of a call: row tiles of 16, blocks of them, splits of the
 // long axis with at most `max_floats` of workspace.

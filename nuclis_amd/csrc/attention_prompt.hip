@@ -1,0 +1,250 @@
+// Attention of many new rows (prompts, chunks of them) over the quantised
+// cache: the formulas, operands and precision of attention.hip, with the cache
+// decoded once for the workgroup.
+//
+// Four waves hold 16 * RT query rows each. A step of TOKENS tokens is decoded to
+// f16 operands in LDS by all four (each a quarter of K's and of V's operands,
+// as one lane's wide load gives them), and read by all four: an operand is 64
+// lanes of 16 bytes in lane order, so writes and reads are linear and free of
+// bank conflicts. Two LDS buffers and one register stage: while a step is
+// computed, the next is decoded from registers into the other buffer and the one
+// after it is on its way from memory; one barrier a step.
+//
+// Why decoded through LDS: a step of 64 tokens costs about 400 vector
+// instructions to decode, as many as the softmax of 64 rows; shared by four waves
+// it is a quarter. RT is what two workgroups a CU leave room for in registers (O,
+// Q and a step's scores), since one's products then run under the other's softmax.
+#include "attention_tiles.h"
+
+namespace nuq {
+
+namespace {
+
+template <int BITS, int D> struct Step {
+    using G = CacheGeometry<BITS, D>;
+    static constexpr int TOKENS = D == 256 ? 32 : 64;  // 64 KB of LDS at D = 128 and 256
+    static constexpr int TILES = TOKENS / 16, PAIRS = TOKENS / 32;
+    static constexpr int K_ITEMS = TILES * G::UNITS / WAVES;      // (tile, unit)s a wave decodes
+    static constexpr int V_ITEMS = PAIRS * (D / 16) / WAVES;      // V operands, all of one (pair, unit)
+    static constexpr int WORDS = G::CHUNK / 4;
+    static constexpr int K_OPERANDS = TILES * G::GROUPS, V_OPERANDS = PAIRS * (D / 16);
+    static_assert(K_ITEMS * WAVES == TILES * G::UNITS && V_ITEMS * WAVES == V_OPERANDS, "a wave's share is whole");
+    static_assert(G::COLUMN % V_ITEMS == 0, "a wave's V operands share a unit");
+};
+
+// A wave's share of a step between memory and LDS.
+template <int BITS, int D> struct Raw {
+    using S = Step<BITS, D>;
+    using G = CacheGeometry<BITS, D>;
+    uint32_t k[S::K_ITEMS][S::WORDS], ks[S::K_ITEMS][G::UNIT_GROUPS / 2];
+    uint32_t v[2][S::WORDS], vs[2][2];
+    int v_first[2];                     // this lane's first token of each tile
+    bool k_valid[S::K_ITEMS], v_valid[2];
+
+    __device__ __forceinline__ void load(const CacheView &c, const int32_t *table, uint32_t head, int step, int to,
+                                         int wave, int n, int h) {
+        // tiles past the last token read the step's first tile: they are masked
+        const int first_tile = step * S::TILES;
+        const auto place = [&](int tile, bool &valid) {
+            const bool inside = 16 * (first_tile + tile) < to;
+            return tile_at<BITS, D>(c, table, head, (uint32_t)(inside ? first_tile + tile : first_tile), valid);
+        };
+#pragma unroll
+        for (int i = 0; i < S::K_ITEMS; ++i) {
+            const int item = wave * S::K_ITEMS + i, u = item % G::UNITS;
+            const uint8_t *p = place(item / G::UNITS, k_valid[i]);
+            load_words<G::CHUNK>(k[i], p + ((u * 16 + n) * 4 + h) * G::CHUNK);
+            load_words<2 * G::UNIT_GROUPS>(ks[i], p + G::K_SCALES + 2 * (n * G::GROUPS + u * G::UNIT_GROUPS));
+        }
+        const int operand = wave * S::V_ITEMS, pair = operand / (D / 16), u = operand % (D / 16) / G::COLUMN;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint8_t *p = place(2 * pair + i, v_valid[i]);
+            load_words<G::CHUNK>(v[i], p + G::V_CODES + ((u * 4 + h) * 16 + n) * G::CHUNK);
+            const int group = u * G::UNIT_GROUPS + n * G::COLUMN / 32;
+            load_words<8>(vs[i], p + G::V_SCALES + 8 * (h * G::GROUPS + group));
+            v_first[i] = 16 * (first_tile + 2 * pair + i) + 4 * h;
+        }
+    }
+
+    // `edge`: some token of the step may be unwritten or on no page.
+    __device__ __forceinline__ void decode(uint4 (*kb)[64], uint4 (*vb)[64], int from, int to, bool edge, int wave,
+                                           int lane) {
+#pragma unroll
+        for (int i = 0; i < S::K_ITEMS; ++i) {
+            const int item = wave * S::K_ITEMS + i, tile = item / G::UNITS, u = item % G::UNITS;
+#pragma unroll
+            for (int g = 0; g < G::UNIT_GROUPS; ++g) {
+                const half2v s = as_half2(ks[i][g >> 1]), d = {s[g & 1], s[g & 1]}, b = bias_of<BITS>(d);
+                Operand o;
+                if constexpr (BITS == 4) o = decode_k4(k[i][g], d, b);
+                else o = decode_k8(k[i][2 * g], k[i][2 * g + 1], d, b);
+                kb[tile * G::GROUPS + u * G::UNIT_GROUPS + g][lane] = make_uint4(o.w[0], o.w[1], o.w[2], o.w[3]);
+            }
+        }
+        const int operand = wave * S::V_ITEMS, j0 = operand % G::COLUMN;
+        uint32_t out[4][S::V_ITEMS];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const int i = x >> 1, pair = x & 1;
+            uint32_t scales = vs[i][pair];
+            if (edge) {
+                const int t = v_first[i] + 2 * pair, end = v_valid[i] ? to : 0;
+                uint32_t mask = 0;
+                if (t >= from && t < end) mask |= 0xffffu;
+                if (t + 1 >= from && t + 1 < end) mask |= 0xffff0000u;
+                scales &= mask;
+            }
+            const half2v d = as_half2(scales), b = bias_of<BITS>(d);
+            if constexpr (BITS == 4) {
+                uint32_t w;  // four dimensions of two tokens, from j0 (0 or 4; 0 or 2 at D = 64)
+                if constexpr (G::COLUMN == 8)
+                    w = __builtin_amdgcn_perm(v[i][2 * pair + 1], v[i][2 * pair], j0 ? 0x07060302u : 0x05040100u);
+                else
+                    w = v[i][pair] >> (4 * j0);
+                out[x][0] = as_u32(as_half2(nibbles<0>(w)) * d + b);
+                out[x][1] = as_u32(as_half2(nibbles<1>(w)) * d + b);
+                if constexpr (S::V_ITEMS == 4) {
+                    out[x][2] = as_u32(as_half2(nibbles<2>(w)) * d + b);
+                    out[x][3] = as_u32(as_half2(nibbles<3>(w)) * d + b);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < S::V_ITEMS; ++j) {
+                    const uint32_t pick = 0x0c040c00u + 0x00010001u * (uint32_t)(j0 + j);
+                    const uint32_t w = __builtin_amdgcn_perm(v[i][2 * pair + 1], v[i][2 * pair], pick);
+                    out[x][j] = as_u32(as_half2(w | 0x64006400u) * d + b);
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < S::V_ITEMS; ++j)
+            vb[operand + j][lane] = make_uint4(out[0][j], out[1][j], out[2][j], out[3][j]);
+    }
+};
+
+template <int BITS, int D, int RT, bool F32>
+__global__ void __launch_bounds__(64 * WAVES, 2) attention_prompt_kernel(CacheView c, AttentionArgs a) {
+    using G = CacheGeometry<BITS, D>;
+    using S = Step<BITS, D>;
+    using T = std::conditional_t<F32, float, _Float16>;
+    constexpr int PARTS = F32 ? 2 : 1;
+    __shared__ uint4 kb[2][S::K_OPERANDS][64], vb[2][S::V_OPERANDS][64];
+    __shared__ int valid[2][4];  // of a buffer's tiles
+
+    const int lane = (int)threadIdx.x & 63, n = lane & 15, h = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    uint32_t id = blockIdx.x;  // as in attention_rows_kernel
+    const uint32_t head = id % c.kv_heads;
+    id /= c.kv_heads;
+    const uint32_t split = id % a.splits;
+    id /= a.splits;
+    const uint32_t block = a.blocks - 1 - id % a.blocks, b = id / a.blocks;
+    Span s;
+    if (!span_of<16 * RT * WAVES, S::TOKENS>(a, b, block, split, s)) return;
+    const int32_t *table = a.table + b * a.table_stride;
+
+    const int first_row = s.first_row + 16 * RT * wave;
+    Rows<BITS, D, RT, F32> rows;
+    rows.load(a, s, head, first_row, n, h);
+
+    Raw<BITS, D> raw;
+    const auto decode = [&](int step, int buffer) {
+        const int first = S::TOKENS * step;
+#pragma unroll
+        for (int i = 0; i < S::K_ITEMS; ++i)
+            if (lane == 0) valid[buffer][(wave * S::K_ITEMS + i) / G::UNITS] = raw.k_valid[i];
+        const bool edge = first < s.from || first + S::TOKENS > s.to || !raw.v_valid[0] || !raw.v_valid[1];
+        raw.decode(kb[buffer], vb[buffer], s.from, s.to, edge, wave, lane);
+    };
+    if (s.low < s.high) {
+        raw.load(c, table, head, s.low, s.to, wave, n, h);
+        decode(s.low, 0);
+        if (s.low + 1 < s.high) raw.load(c, table, head, s.low + 1, s.to, wave, n, h);
+        __syncthreads();
+    }
+    for (int step = s.low; step < s.high; ++step) {
+        const int buffer = (step - s.low) & 1, first = S::TOKENS * step;
+        if (step + 1 < s.high) {
+            decode(step + 1, buffer ^ 1);
+            if (step + 2 < s.high) raw.load(c, table, head, step + 2, s.to, wave, n, h);
+        }
+        if (first < rows.seen_to && first + S::TOKENS > rows.seen_from) {
+            int there[S::TILES];
+            bool all = true;
+#pragma unroll
+            for (int i = 0; i < S::TILES; ++i) {
+                there[i] = __builtin_amdgcn_readfirstlane(valid[buffer][i]);
+                all &= there[i] != 0;
+            }
+            const bool masked = first < rows.clear_from || first + S::TOKENS > rows.clear_to || !all;
+#pragma unroll
+            for (int pair = 0; pair < S::PAIRS; ++pair) {
+                floatx4 x[2][RT];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                    for (int t = 0; t < RT; ++t) x[i][t] = floatx4{0, 0, 0, 0};
+#pragma unroll
+                    for (int g = 0; g < G::GROUPS; ++g)
+                        rows.score(__builtin_bit_cast(half8, kb[buffer][(2 * pair + i) * G::GROUPS + g][lane]), g, x[i]);
+                }
+                if (masked) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) rows.mask(x[i], first + 32 * pair + 16 * i + 4 * h, there[2 * pair + i]);
+                }
+                Operand p[PARTS][RT];
+                rows.weigh(x[0], x[1], p);
+#pragma unroll
+                for (int j = 0; j < D / 16; ++j)
+                    rows.add(__builtin_bit_cast(half8, vb[buffer][pair * (D / 16) + j][lane]), j, p);
+            }
+        }
+        __syncthreads();
+    }
+
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const float l = over_quarters_sum(rows.sum[t]);
+        const int row = first_row + 16 * t + n;
+        if (row >= s.rows) continue;
+        const int token = row / (int)a.group;
+        const uint64_t out_row = (uint64_t)(s.start + token);
+        const uint32_t out_head = head * a.group + row - token * a.group;
+        const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+        const uint64_t at = (out_row * (c.kv_heads * a.group) + out_head) * a.splits + split;
+        if (a.splits > 1 && h == 0) a.partial_ml[2 * at] = rows.top[t], a.partial_ml[2 * at + 1] = l;
+#pragma unroll
+        for (int u = 0; u < G::UNITS; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int j = 0; j < G::COLUMN; j += 4) {
+                    const int o = u * G::COLUMN + j, dim = u * G::UNIT_DIMS + (4 * h + e) * G::COLUMN + j;
+                    const float4 x = make_float4(rows.o[t][o][e], rows.o[t][o + 1][e], rows.o[t][o + 2][e],
+                                                 rows.o[t][o + 3][e]);
+                    if (a.splits > 1) *(float4 *)(a.partial_o + at * D + dim) = x;
+                    else store4((T *)a.out + out_row * a.out_stride + out_head * D + dim, x, inverse);
+                }
+    }
+}
+
+template <int BITS, int D, bool F32> hipError_t prompt_launch(hipStream_t s, const CacheView &c, const AttentionArgs &a) {
+    constexpr int RT = prompt_row_tiles(D, F32);
+    const uint32_t grid = c.kv_heads * a.splits * a.blocks * a.batch;
+    attention_prompt_kernel<BITS, D, RT, F32><<<grid, 64 * WAVES, 0, s>>>(c, a);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_attention_prompt(hipStream_t s, const CacheView &c, uint32_t bits, uint32_t d, uint32_t f32,
+                                   const AttentionArgs &a) {
+#define NUQ_CASE(B, D) \
+    if (bits == B && d == D) return f32 ? prompt_launch<B, D, true>(s, c, a) : prompt_launch<B, D, false>(s, c, a);
+    NUQ_CASE(4, 64) NUQ_CASE(4, 128) NUQ_CASE(4, 256) NUQ_CASE(8, 64) NUQ_CASE(8, 128) NUQ_CASE(8, 256)
+#undef NUQ_CASE
+    return hipErrorInvalidValue;
+}
+
+}  // namespace nuq
