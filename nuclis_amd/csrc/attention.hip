@@ -39,13 +39,27 @@ namespace nuq {
 
 namespace {
 
-constexpr int STEP = 32;  // tokens a wave takes at a time
-
+// Registers of a wave beside its steps in work and on their way: O, Q, and a step's scores, weights and decoded V.
+constexpr int held_registers(int bits, int d, int rt, bool f32, int tiles) {
+    const int parts = f32 ? 2 : 1, column = bits == 4 && d > 64 ? 8 : 4;
+    return rt * d / 4 + rt * parts * d / 8 + tiles * (4 * rt + 2 * rt * parts + 2 * column) + 30;
+}
+// A tile's registers (struct Tile).
+constexpr int tile_registers(int bits, int d) {
+    const int units = d * bits / 32 <= 16 ? 1 : d * bits / 512;
+    return 2 * (d * bits / 128) + d / 64 + 2 * units;
+}
+// A wave's step is two tiles of 16 tokens, or one where two such steps on their
+// way do not fit 256 registers (two waves a SIMD).
+constexpr int step_tiles(int bits, int d, int rt, bool f32) {
+    return held_registers(bits, d, rt, f32, 2) + 4 * tile_registers(bits, d) <= 240 ? 2 : 1;
+}
 template <int BITS, int D, int RT, bool F32>
 __global__ void __launch_bounds__(64 * WAVES, 2) attention_rows_kernel(CacheView c, AttentionArgs a) {
     using G = CacheGeometry<BITS, D>;
     using T = std::conditional_t<F32, float, _Float16>;
     constexpr int PARTS = F32 ? 2 : 1;
+    constexpr int TILES = step_tiles(BITS, D, RT, F32), STEP = 16 * TILES;
     __shared__ __align__(16) float merge_o[WAVES][16][D + 4];
     __shared__ float merge_m[WAVES][16], merge_l[WAVES][16];
 
@@ -61,60 +75,84 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_rows_kernel(CacheView
     const uint32_t block = a.blocks - 1 - id % a.blocks, b = id / a.blocks;  // long rows first
     Span s;
     if (!span_of<16 * RT, STEP>(a, b, block, split, s)) return;
-    const int32_t *table = a.table + b * a.table_stride;
+    const PageTable table = table_of(a, b);
 
     Rows<BITS, D, RT, F32> rows;
-    rows.load(a, s, head, s.first_row, n, h);
+    typename Rows<BITS, D, RT, F32>::Raw queries;
+    rows.load(a, s, head, s.first_row, n, h, queries);
 
-    Tile<BITS, D> next[2];
-    bool next_valid[2];
-    const auto fetch = [&](int step) {
-        // the second half of the last step may lie past the table: it is masked, and reads the first half again
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int tile = 2 * step + i;
-            const bool inside = 16 * tile < s.to;
-            next[i].load(tile_at<BITS, D>(c, table, head, (uint32_t)(inside ? tile : 2 * step), next_valid[i]), n, h);
-        }
+    // Two steps ahead a wave looks up the pages, one step ahead it requests the tiles. The
+    // second half of the last step may lie past the table: it is masked, and reads the first half again.
+    Tile<BITS, D> next[TILES];
+    bool next_valid[TILES];
+    uint32_t page[TILES];
+    const auto tile_of = [&](int step, int i) {
+        const int first = TILES * step;
+        return (uint32_t)(16 * (first + i) < s.to ? first + i : first);
     };
-    int step = s.low + wave;
-    if (step < s.high) fetch(step);
-    for (; step < s.high; step += WAVES) {
-        Tile<BITS, D> tile[2] = {next[0], next[1]};
-        const bool valid[2] = {next_valid[0], next_valid[1]};
-        if (step + WAVES < s.high) fetch(step + WAVES);
-
-        floatx4 x[2][RT];
+    const auto look_up = [&](int step) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < TILES; ++i) page[i] = (uint32_t)table[tile_of(step, i) >> c.tiles_log2];
+    };
+    const auto fetch = [&](int step) {
+#pragma unroll
+        for (int i = 0; i < TILES; ++i)
+            next[i].load(tile_at<BITS, D>(c, page[i], head, tile_of(step, i), next_valid[i]), n, h);
+    };
+    const int first_step = s.low + wave;
+    // (the queries' F32 values and a step under way do not fit where rows are many or wide)
+    if constexpr (F32 && RT * D > 128) rows.prepare(queries);
+    // Loads stand under no condition, so that the compiler knows what to wait for:
+    // past its last step a wave asks for that one again.
+    const int last = max(s.high - 1, 0);
+    look_up(min(first_step, last));
+    fetch(min(first_step, last));
+    look_up(min(first_step + WAVES, last));
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (!F32 || RT * D <= 128) rows.prepare(queries);
+    for (int step = first_step; step < s.high; step += WAVES) {
+        Tile<BITS, D> tile[TILES];
+        bool valid[TILES];
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) tile[i] = next[i], valid[i] = next_valid[i];
+        fetch(min(step + WAVES, last));
+        look_up(min(step + 2 * WAVES, last));
+        floatx4 x[TILES][RT];
+        bool whole = true;
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) {
+            whole &= valid[i];
 #pragma unroll
             for (int t = 0; t < RT; ++t) x[i][t] = floatx4{0, 0, 0, 0};
 #pragma unroll
             for (int g = 0; g < G::GROUPS; ++g)
-                rows.score(tile[i].k_operand(g / G::UNIT_GROUPS, g % G::UNIT_GROUPS, tile[i].k_scale(g)).get(), g, x[i]);
+                rows.score(tile[i].k_operand(g / G::UNIT_GROUPS, g % G::UNIT_GROUPS, tile[i].k_scale(g)).get(), g,
+                           x[i]);
         }
-        if (STEP * step < rows.clear_from || STEP * (step + 1) > rows.clear_to || !valid[0] || !valid[1]) {
+        if (STEP * step < rows.clear_from || STEP * (step + 1) > rows.clear_to || !whole) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < TILES; ++i) {
                 const int first = STEP * step + 16 * i + 4 * h;
                 rows.mask(x[i], first, valid[i]);
                 tile[i].keep(first, s.from, valid[i] ? s.to : 0);
             }
         }
         Operand p[PARTS][RT];
-        rows.weigh(x[0], x[1], p);
+        rows.template weigh<TILES>(x, p);
 #pragma unroll
         for (int u = 0; u < G::UNITS; ++u) {
-            uint32_t v[4][G::COLUMN];
+            uint32_t v[2 * TILES][G::COLUMN];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const half2v d = as_half2(tile[k >> 1].vs[u][k & 1]);
-                decode_v<BITS, G::COLUMN>(tile[k >> 1].v[u], k & 1, d, bias_of<BITS>(d), v[k]);
+            for (int i = 0; i < 2 * TILES; ++i) {
+                const half2v d = as_half2(tile[i >> 1].vs[u][i & 1]);
+                decode_v<BITS, G::COLUMN>(tile[i >> 1].v[u], i & 1, d, bias_of<BITS>(d), v[i]);
             }
 #pragma unroll
             for (int j = 0; j < G::COLUMN; ++j) {
-                const Operand av = {{v[0][j], v[1][j], v[2][j], v[3][j]}};
-                rows.add(av.get(), u * G::COLUMN + j, p);
+                Operand av;
+#pragma unroll
+                for (int i = 0; i < 2 * TILES; ++i) av.w[i] = v[i][j];
+                rows.template add<TILES>(av, u * G::COLUMN + j, p);
             }
         }
     }
@@ -176,8 +214,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_rows_kernel(CacheView
 
 // Joins the splits of one (sequence, token, head) a workgroup: the first wave
 // turns the splits' maxima into weights, then D / 4 threads take a split, 1024 / D
-// splits at a time. A split without a token has sum 0 and no output: it is not
-// read. (One wave walking 64 splits in order took 29 us after 32768 tokens,
+// splits at a time. (A split without a token has sum 0 and zeros. One wave walking 64 splits in order took 29 us after 32768 tokens,
 // one round of memory latency a split; this takes 3.9.)
 template <int D, bool F32>
 __global__ void __launch_bounds__(256) attention_join_kernel(AttentionArgs a, uint32_t heads) {
@@ -203,7 +240,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(AttentionArgs a, ui
         float sum = l == 0.0f ? 0.0f : w * l;
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
-        weight[tid] = l == 0.0f ? -1.0f : w;
+        weight[tid] = w;
         if (tid == 0) total = sum;
     }
     __syncthreads();
@@ -213,8 +250,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(AttentionArgs a, ui
 #pragma unroll 4
     for (uint32_t i = side; i < a.splits; i += SIDE) {
         const float w = weight[i];
-        float4 y = make_float4(0, 0, 0, 0);
-        if (w != -1.0f) y = *(const float4 *)(p + (uint64_t)i * D);
+        const float4 y = *(const float4 *)(p + (uint64_t)i * D);
         x.x += w * y.x, x.y += w * y.y, x.z += w * y.z, x.w += w * y.w;
     }
     *(float4 *)&part[side][x4] = x;

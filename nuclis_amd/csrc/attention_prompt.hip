@@ -41,28 +41,30 @@ template <int BITS, int D> struct Raw {
     int v_first[2];                     // this lane's first token of each tile
     bool k_valid[S::K_ITEMS], v_valid[2];
 
-    __device__ __forceinline__ void load(const CacheView &c, const int32_t *table, uint32_t head, int step, int to,
+    __device__ __forceinline__ void load(const CacheView &c, PageTable table, uint32_t head, int step, int to,
                                          int wave, int n, int h) {
         // tiles past the last token read the step's first tile: they are masked
         const int first_tile = step * S::TILES;
         const auto place = [&](int tile, bool &valid) {
             const bool inside = 16 * (first_tile + tile) < to;
-            return tile_at<BITS, D>(c, table, head, (uint32_t)(inside ? first_tile + tile : first_tile), valid);
+            return tile_at<BITS, D>(c, (uint32_t)table[(uint32_t)(first_tile + (inside ? tile : 0)) >> c.tiles_log2], head,
+                                    (uint32_t)(first_tile + (inside ? tile : 0)), valid);
         };
 #pragma unroll
         for (int i = 0; i < S::K_ITEMS; ++i) {
             const int item = wave * S::K_ITEMS + i, u = item % G::UNITS;
             const uint8_t *p = place(item / G::UNITS, k_valid[i]);
-            load_words<G::CHUNK>(k[i], p + ((u * 16 + n) * 4 + h) * G::CHUNK);
-            load_words<2 * G::UNIT_GROUPS>(ks[i], p + G::K_SCALES + 2 * (n * G::GROUPS + u * G::UNIT_GROUPS));
+            load_words<G::CHUNK>(k[i], p + u * 64 * G::CHUNK, (uint32_t)(n * 4 + h) * G::CHUNK);
+            load_words<2 * G::UNIT_GROUPS>(ks[i], p + G::K_SCALES + 2 * u * G::UNIT_GROUPS,
+                                           (uint32_t)(2 * n * G::GROUPS));
         }
         const int operand = wave * S::V_ITEMS, pair = operand / (D / 16), u = operand % (D / 16) / G::COLUMN;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const uint8_t *p = place(2 * pair + i, v_valid[i]);
-            load_words<G::CHUNK>(v[i], p + G::V_CODES + ((u * 4 + h) * 16 + n) * G::CHUNK);
-            const int group = u * G::UNIT_GROUPS + n * G::COLUMN / 32;
-            load_words<8>(vs[i], p + G::V_SCALES + 8 * (h * G::GROUPS + group));
+            load_words<G::CHUNK>(v[i], p + G::V_CODES + u * 64 * G::CHUNK, (uint32_t)(h * 16 + n) * G::CHUNK);
+            load_words<8>(vs[i], p + G::V_SCALES + 8 * u * G::UNIT_GROUPS,
+                          (uint32_t)(8 * (h * G::GROUPS + n * G::COLUMN / 32)));
             v_first[i] = 16 * (first_tile + 2 * pair + i) + 4 * h;
         }
     }
@@ -142,11 +144,12 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_prompt_kernel(CacheVi
     const uint32_t block = a.blocks - 1 - id % a.blocks, b = id / a.blocks;
     Span s;
     if (!span_of<16 * RT * WAVES, S::TOKENS>(a, b, block, split, s)) return;
-    const int32_t *table = a.table + b * a.table_stride;
+    const PageTable table = table_of(a, b);
 
     const int first_row = s.first_row + 16 * RT * wave;
     Rows<BITS, D, RT, F32> rows;
-    rows.load(a, s, head, first_row, n, h);
+    typename Rows<BITS, D, RT, F32>::Raw queries;
+    rows.load(a, s, head, first_row, n, h, queries);
 
     Raw<BITS, D> raw;
     const auto decode = [&](int step, int buffer) {
@@ -157,17 +160,18 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_prompt_kernel(CacheVi
         const bool edge = first < s.from || first + S::TOKENS > s.to || !raw.v_valid[0] || !raw.v_valid[1];
         raw.decode(kb[buffer], vb[buffer], s.from, s.to, edge, wave, lane);
     };
+    if (s.low < s.high) raw.load(c, table, head, s.low, s.to, wave, n, h);
+    rows.prepare(queries);
     if (s.low < s.high) {
-        raw.load(c, table, head, s.low, s.to, wave, n, h);
         decode(s.low, 0);
-        if (s.low + 1 < s.high) raw.load(c, table, head, s.low + 1, s.to, wave, n, h);
+        raw.load(c, table, head, min(s.low + 1, s.high - 1), s.to, wave, n, h);
         __syncthreads();
     }
     for (int step = s.low; step < s.high; ++step) {
         const int buffer = (step - s.low) & 1, first = S::TOKENS * step;
         if (step + 1 < s.high) {
             decode(step + 1, buffer ^ 1);
-            if (step + 2 < s.high) raw.load(c, table, head, step + 2, s.to, wave, n, h);
+            raw.load(c, table, head, min(step + 2, s.high - 1), s.to, wave, n, h);
         }
         if (first < rows.seen_to && first + S::TOKENS > rows.seen_from) {
             int there[S::TILES];
@@ -194,10 +198,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_prompt_kernel(CacheVi
                     for (int i = 0; i < 2; ++i) rows.mask(x[i], first + 32 * pair + 16 * i + 4 * h, there[2 * pair + i]);
                 }
                 Operand p[PARTS][RT];
-                rows.weigh(x[0], x[1], p);
+                rows.template weigh<2>(x, p);
 #pragma unroll
                 for (int j = 0; j < D / 16; ++j)
-                    rows.add(__builtin_bit_cast(half8, vb[buffer][pair * (D / 16) + j][lane]), j, p);
+                    rows.template add<2>(__builtin_bit_cast(Operand, vb[buffer][pair * (D / 16) + j][lane]), j, p);
             }
         }
         __syncthreads();

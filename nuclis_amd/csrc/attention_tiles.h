@@ -9,6 +9,7 @@ namespace nuq {
 namespace {
 
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 
@@ -20,10 +21,27 @@ constexpr int WAVES = 4, MAX_SPLITS = 64;
 __device__ __forceinline__ half2v as_half2(uint32_t u) { return __builtin_bit_cast(half2v, u); }
 __device__ __forceinline__ uint32_t as_u32(half2v h) { return __builtin_bit_cast(uint32_t, h); }
 
+// What rounding x0, x1 to `hi` left over: x - (float)hi in one instruction each.
+__device__ __forceinline__ half2v rest_of(half2v hi, float x0, float x1) {
+    float a, b;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(a) : "v"(as_u32(hi)), "v"(x0));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(b) : "v"(as_u32(hi)), "v"(x1));
+    return half2v{(_Float16)a, (_Float16)b};
+}
+
 struct Operand {  // 8 f16 of one lane
     uint32_t w[4];
     __device__ __forceinline__ half8 get() const { return __builtin_bit_cast(half8, *this); }
+    __device__ __forceinline__ half4 low() const { return __builtin_shufflevector(get(), get(), 0, 1, 2, 3); }
 };
+
+// (x & mask) | bits as the one instruction it is: it takes one constant from a
+// scalar register, so the compiler, left to itself, keeps both there and issues two.
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
+    uint32_t out;
+    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(out) : "v"(x), "s"(mask), "v"(bits));
+    return out;
+}
 
 // A nibble in the top mantissa bits of 16.0 is 16 + code; a byte under 0x64 is
 // 1024 + code. One f16 fma by (d, -bias d) then gives d * (code - offset) exactly.
@@ -34,7 +52,7 @@ template <int BITS> __device__ __forceinline__ half2v bias_of(half2v d) {
 template <int I> __device__ __forceinline__ uint32_t nibbles(uint32_t w) {
     constexpr int SHIFT = 6 - 4 * I;
     const uint32_t s = SHIFT >= 0 ? w << (SHIFT >= 0 ? SHIFT : 0) : w >> (SHIFT >= 0 ? 0 : -SHIFT);
-    return (s & 0x03c003c0u) | 0x4c004c00u;
+    return and_or(s, 0x03c003c0u, 0x4c004c00u);
 }
 
 // 8 dimensions of one token.
@@ -88,7 +106,11 @@ __device__ __forceinline__ void store4(_Float16 *to, const float4 &x, float by) 
     *(uint2 *)to = make_uint2(as_u32(lo), as_u32(hi));
 }
 
-template <int BYTES> __device__ __forceinline__ void load_words(uint32_t *to, const uint8_t *p) {
+template <int BYTES> __device__ __forceinline__ void load_words(uint32_t *to, const uint8_t *base, uint32_t offset) {
+    // (kept from being widened outside a loop: the load then takes the base from
+    // scalar registers and adds these 32 bits itself)
+    asm volatile("" : "+v"(offset));
+    const uint8_t *p = base + offset;
     if constexpr (BYTES == 16) {
         const uint4 v = *(const uint4 *)p;
         to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
@@ -111,12 +133,12 @@ template <int BITS, int D> struct Tile {
     __device__ __forceinline__ void load(const uint8_t *tile, int n, int h) {
 #pragma unroll
         for (int u = 0; u < G::UNITS; ++u) {
-            load_words<G::CHUNK>(k[u], tile + ((u * 16 + n) * 4 + h) * G::CHUNK);
-            load_words<G::CHUNK>(v[u], tile + G::V_CODES + ((u * 4 + h) * 16 + n) * G::CHUNK);
-            const int group = u * G::UNIT_GROUPS + n * G::COLUMN / 32;
-            load_words<8>(vs[u], tile + G::V_SCALES + 8 * (h * G::GROUPS + group));
+            load_words<G::CHUNK>(k[u], tile + u * 64 * G::CHUNK, (uint32_t)(n * 4 + h) * G::CHUNK);
+            load_words<G::CHUNK>(v[u], tile + G::V_CODES + u * 64 * G::CHUNK, (uint32_t)(h * 16 + n) * G::CHUNK);
+            load_words<8>(vs[u], tile + G::V_SCALES + 8 * u * G::UNIT_GROUPS,
+                          (uint32_t)(8 * (h * G::GROUPS + n * G::COLUMN / 32)));
         }
-        load_words<2 * G::GROUPS>(ks, tile + G::K_SCALES + 2 * n * G::GROUPS);
+        load_words<2 * G::GROUPS>(ks, tile + G::K_SCALES, (uint32_t)(2 * n * G::GROUPS));
     }
     __device__ __forceinline__ half2v k_scale(int g) const {
         const half2v s = as_half2(ks[g >> 1]);
@@ -141,15 +163,23 @@ template <int BITS, int D> struct Tile {
     }
 };
 
-// The tile index's place in the cache; `valid` is false for a page it lacks.
+// A sequence's row of the page table, which nothing writes meanwhile: read by scalar loads.
+typedef const __attribute__((address_space(4))) int32_t *PageTable;
+__device__ __forceinline__ PageTable table_of(const AttentionArgs &a, uint32_t b) {
+    return (PageTable)(uintptr_t)(a.table + b * a.table_stride);
+}
+
+// The place of tile `tile` of its sequence, on page `page`; `valid` is false for a page the cache lacks.
 template <int BITS, int D>
-__device__ __forceinline__ const uint8_t *tile_at(const CacheView &c, const int32_t *__restrict__ table, uint32_t head,
-                                                  uint32_t tile, bool &valid) {
-    const uint32_t page = (uint32_t)table[tile >> c.tiles_log2];
+__device__ __forceinline__ const uint8_t *tile_at(const CacheView &c, uint32_t page, uint32_t head, uint32_t tile,
+                                                  bool &valid) {
     valid = page < c.pages;
     const uint64_t at = (((uint64_t)(valid ? page : 0) * c.kv_heads + head) << c.tiles_log2) +
                         (tile & ((1u << c.tiles_log2) - 1u));
-    return c.bytes + at * CacheGeometry<BITS, D>::TILE_BYTES;
+    // one for the wave, in scalar registers: loads take a 32-bit offset a lane beside it
+    const uint64_t from = at * CacheGeometry<BITS, D>::TILE_BYTES;
+    return c.bytes + ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(from >> 32)) << 32 |
+                      (uint32_t)__builtin_amdgcn_readfirstlane((int)from));
 }
 
 // Over a row's four lanes (quarters h of lane / 16), by swaps of rows of lanes.
@@ -226,40 +256,60 @@ template <int BITS, int D, int RT, bool F32> struct Rows {
     int clear_from, clear_to;      // tokens [clear_from, clear_to) are seen by every live row
     int seen_from, seen_to;        // tokens some live row sees
 
+    // Query rows as they are in memory, before `prepare` makes them operands (F32)
+    // (F16: they are operands as they come).
+    struct Raw {
+        float4 x[F32 ? RT : 1][F32 ? GROUPS : 1][2];
+    };
+
+    // Requests the rows and sets their positions.
     __device__ __forceinline__ void load(const AttentionArgs &a, const Span &s, uint32_t head, int first_row, int n,
-                                         int h) {
+                                         int h, Raw &raw) {
         const int group = (int)a.group;
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-            const int row = first_row + 16 * t + n, token = row / group;
-            const bool live = row < s.rows;
+            // (rows past the last are its copies: their results are not written, and loads
+            // without a branch around them leave the compiler exact counts to wait for)
+            const int row = min(first_row + 16 * t + n, s.rows - 1), token = row / group;
             const T *p = (const T *)a.q + (uint64_t)(s.start + token) * a.q_stride +
                          (head * a.group + row - token * group) * D;
-            position[t] = live ? s.position + token : -1;
+            position[t] = s.position + token;
             below[t] = a.window ? s.position + token - (int)a.window : -1;
             scale[t] = a.scale;
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) {
+                if constexpr (F32) {
+                    raw.x[t][g][0] = ((const float4 *)(p + 32 * g + 8 * h))[0];
+                    raw.x[t][g][1] = ((const float4 *)(p + 32 * g + 8 * h))[1];
+                } else {
+                    const uint4 v = *(const uint4 *)(p + 32 * g + 8 * h);
+                    q[0][t][g] = {{v.x, v.y, v.z, v.w}};
+                }
+            }
+        }
+        const int low = s.position + min(first_row, s.rows - 1) / group;
+        const int high = s.position + (min(first_row + 16 * RT, s.rows) - 1) / group;
+        clear_to = low + 1;
+        clear_from = a.window ? max(high - (int)a.window + 1, 0) : 0;
+        seen_to = first_row < s.rows ? high + 1 : 0;
+        seen_from = a.window ? max(low - (int)a.window + 1, 0) : 0;
+    }
+
+    __device__ __forceinline__ void prepare(const Raw &raw) {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
             top[t] = LOWEST, sum[t] = 0.0f;
 #pragma unroll
             for (int j = 0; j < TILES_O; ++j) o[t][j] = floatx4{0, 0, 0, 0};
-            if constexpr (!F32) {
-#pragma unroll
-                for (int g = 0; g < GROUPS; ++g) {
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (live) v = *(const uint4 *)(p + 32 * g + 8 * h);
-                    q[0][t][g] = {{v.x, v.y, v.z, v.w}};
-                }
-            } else {
-                float x[GROUPS][8];
+            if constexpr (F32) {
                 float most = 0.0f;
 #pragma unroll
-                for (int g = 0; g < GROUPS; ++g) {
-                    float4 u = make_float4(0, 0, 0, 0), v = u;
-                    if (live) u = ((const float4 *)(p + 32 * g + 8 * h))[0], v = ((const float4 *)(p + 32 * g + 8 * h))[1];
-                    x[g][0] = u.x, x[g][1] = u.y, x[g][2] = u.z, x[g][3] = u.w;
-                    x[g][4] = v.x, x[g][5] = v.y, x[g][6] = v.z, x[g][7] = v.w;
+                for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[g][e]));
-                }
+                    for (int i = 0; i < 2; ++i) {
+                        const float4 &x = raw.x[t][g][i];
+                        most = fmaxf(fmaxf(fmaxf(most, fabsf(x.x)), fmaxf(fabsf(x.y), fabsf(x.z))), fabsf(x.w));
+                    }
                 // the row's largest magnitude comes to [2^7, 2^8): hi + lo then hold 22 bits of it
                 most = over_quarters_max(most);
                 const uint32_t exponent = min(max(__float_as_uint(most) >> 23 & 255u, 8u), 254u);
@@ -270,20 +320,15 @@ template <int BITS, int D, int RT, bool F32> struct Rows {
                 for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float x0 = x[g][2 * e] * up, x1 = x[g][2 * e + 1] * up;
+                        const float4 &x = raw.x[t][g][e >> 1];
+                        const float x0 = ((e & 1) ? x.z : x.x) * up, x1 = ((e & 1) ? x.w : x.y) * up;
                         const half2v hi = {(_Float16)x0, (_Float16)x1};
-                        const half2v lo = {(_Float16)(x0 - (float)hi[0]), (_Float16)(x1 - (float)hi[1])};
+                        const half2v lo = rest_of(hi, x0, x1);
                         q[0][t][g].w[e] = as_u32(hi);
                         q[PARTS - 1][t][g].w[e] = as_u32(lo);
                     }
             }
         }
-        const int low = s.position + first_row / group;
-        const int high = s.position + (min(first_row + 16 * RT, s.rows) - 1) / group;
-        clear_to = low + 1;
-        clear_from = a.window ? max(high - (int)a.window + 1, 0) : 0;
-        seen_to = first_row < s.rows ? high + 1 : 0;
-        seen_from = a.window ? max(low - (int)a.window + 1, 0) : 0;
     }
 
     // S^T += K Q^T of one group
@@ -294,13 +339,17 @@ template <int BITS, int D, int RT, bool F32> struct Rows {
             for (int p = 0; p < PARTS; ++p)
                 x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[p][t][g].get(), x[t], 0, 0, 0);
     }
-    // O^T += V^T P^T of 16 dimensions
-    __device__ __forceinline__ void add(half8 v, int j, const Operand (&p)[PARTS][RT]) {
+    // O^T += V^T P^T of 16 dimensions, over two tiles' tokens (k = 32) or one's (k = 16)
+    template <int TILES> __device__ __forceinline__ void add(const Operand &v, int j, const Operand (&p)[PARTS][RT]) {
 #pragma unroll
         for (int t = 0; t < RT; ++t)
 #pragma unroll
-            for (int i = 0; i < PARTS; ++i)
-                o[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[i][t].get(), o[t][j], 0, 0, 0);
+            for (int i = 0; i < PARTS; ++i) {
+                if constexpr (TILES == 2)
+                    o[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v.get(), p[i][t].get(), o[t][j], 0, 0, 0);
+                else
+                    o[t][j] = __builtin_amdgcn_mfma_f32_16x16x16f16(v.low(), p[i][t].low(), o[t][j], 0, 0, 0);
+            }
     }
     // Scores of the tokens first .. first + 3 (this lane's) that a row does not see become -inf.
     // (Bitwise on purpose: one select a score, no branches.)
@@ -315,14 +364,17 @@ template <int BITS, int D, int RT, bool F32> struct Rows {
             }
         }
     }
-    // Weights of two tiles' raw scores, as the B operand of the next product.
+    // Weights of one or two tiles' raw scores as the B operand of the next product.
     // The common step asks only whether any score passes its row's reference by
     // more than SLACK; the maximum over the row's lanes is taken where one does.
-    __device__ __forceinline__ void weigh(const floatx4 (&a)[RT], const floatx4 (&b)[RT], Operand (&p)[PARTS][RT]) {
+    template <int TILES> __device__ __forceinline__ void weigh(const floatx4 (&x)[TILES][RT], Operand (&p)[PARTS][RT]) {
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-            float most = fmaxf(fmaxf(fmaxf(a[t][0], a[t][1]), fmaxf(a[t][2], a[t][3])),
-                               fmaxf(fmaxf(b[t][0], b[t][1]), fmaxf(b[t][2], b[t][3]))) * scale[t];
+            float most = -__builtin_inff();
+#pragma unroll
+            for (int i = 0; i < TILES; ++i)
+                most = fmaxf(most, fmaxf(fmaxf(x[i][t][0], x[i][t][1]), fmaxf(x[i][t][2], x[i][t][3])));
+            most *= scale[t];
             if (__any(most > top[t] + SLACK)) {
                 most = over_quarters_max(most);
                 const float higher = fmaxf(top[t], most), by = __builtin_amdgcn_exp2f(top[t] - higher);
@@ -332,18 +384,17 @@ template <int BITS, int D, int RT, bool F32> struct Rows {
                 for (int j = 0; j < TILES_O; ++j) o[t][j] *= by;
             }
             const float down = RAISE - top[t];
-            float w[8];
+            float w[4 * TILES];
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(e < 4 ? a[t][e & 3] : b[t][e & 3], scale[t], down));
-            sum[t] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+            for (int e = 0; e < 4 * TILES; ++e)
+                w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e >> 2][t][e & 3], scale[t], down));
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
+            for (int i = 0; i < TILES; ++i) sum[t] += (w[4 * i] + w[4 * i + 1]) + (w[4 * i + 2] + w[4 * i + 3]);
+#pragma unroll
+            for (int e = 0; e < 2 * TILES; ++e) {
                 const half2v hi = {(_Float16)w[2 * e], (_Float16)w[2 * e + 1]};
                 p[0][t].w[e] = as_u32(hi);
-                if constexpr (F32)
-                    p[PARTS - 1][t].w[e] = as_u32(half2v{(_Float16)(w[2 * e] - (float)hi[0]),
-                                                         (_Float16)(w[2 * e + 1] - (float)hi[1])});
+                if constexpr (F32) p[PARTS - 1][t].w[e] = as_u32(rest_of(hi, w[2 * e], w[2 * e + 1]));
             }
         }
     }
