@@ -304,12 +304,16 @@ void plan_attention(uint32_t bits, uint32_t head_dim, uint32_t kv_heads, uint32_
     const uint64_t groups = (uint64_t)a->batch * kv_heads * a->blocks;
     uint64_t reach = max_length;
     if (a->window) reach = std::min<uint64_t>(reach, (uint64_t)a->window + a->max_tokens);
-    // enough workgroups for two on every CU, each with at least one step a wave
-    // (the prompt kernel: four steps a workgroup)
-    const uint64_t least = a->prompt ? 256 : 128;
-    uint64_t splits = std::max<uint64_t>(1, std::min<uint64_t>((512 + groups - 1) / groups, (reach + least - 1) / least));
-    splits = std::min<uint64_t>(splits, MAX_SPLITS);
-    if (a->prompt && groups >= 256) splits = 1;
+    uint64_t splits = 1;
+    if (a->prompt) {
+        splits = std::min((768 + groups - 1) / groups, (reach + 255) / 256);
+        if (groups >= 768) splits = 1;
+    } else if (reach > 512) {
+        const uint64_t short_ones = std::min(256 / groups, (reach + 127) / 128);
+        const uint64_t long_ones = std::min(1024 / groups, reach / 1024);
+        splits = std::max(short_ones, long_ones);
+    }
+    splits = std::max<uint64_t>(1, std::min<uint64_t>(splits, MAX_SPLITS));
     const uint64_t each = (uint64_t)a->rows * heads * (head_dim + 2);
     if (splits > 1 && splits * each > max_floats) splits = std::max<uint64_t>(1, max_floats / each);
     a->splits = (uint32_t)splits;

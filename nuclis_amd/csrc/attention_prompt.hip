@@ -38,22 +38,24 @@ template <int BITS, int D> struct Raw {
     using G = CacheGeometry<BITS, D>;
     uint32_t k[S::K_ITEMS][S::WORDS], ks[S::K_ITEMS][G::UNIT_GROUPS / 2];
     uint32_t v[2][S::WORDS], vs[2][2];
-    int v_first[2];                     // this lane's first token of each tile
-    bool k_valid[S::K_ITEMS], v_valid[2];
+    uint32_t there;                     // bit i: the i-th K item's page exists; bits 30, 31: V's tiles' do
 
     __device__ __forceinline__ void load(const CacheView &c, PageTable table, uint32_t head, int step, int to,
                                          int wave, int n, int h) {
         // tiles past the last token read the step's first tile: they are masked
         const int first_tile = step * S::TILES;
-        const auto place = [&](int tile, bool &valid) {
-            const bool inside = 16 * (first_tile + tile) < to;
-            return tile_at<BITS, D>(c, (uint32_t)table[(uint32_t)(first_tile + (inside ? tile : 0)) >> c.tiles_log2], head,
-                                    (uint32_t)(first_tile + (inside ? tile : 0)), valid);
+        const auto place = [&](int tile, int bit) {
+            const uint32_t at = (uint32_t)(first_tile + (16 * (first_tile + tile) < to ? tile : 0));
+            bool valid;
+            const uint8_t *p = tile_at<BITS, D>(c, (uint32_t)table[at >> c.tiles_log2], head, at, valid);
+            there |= (uint32_t)valid << bit;
+            return p;
         };
+        there = 0;
 #pragma unroll
         for (int i = 0; i < S::K_ITEMS; ++i) {
             const int item = wave * S::K_ITEMS + i, u = item % G::UNITS;
-            const uint8_t *p = place(item / G::UNITS, k_valid[i]);
+            const uint8_t *p = place(item / G::UNITS, i);
             load_words<G::CHUNK>(k[i], p + u * 64 * G::CHUNK, (uint32_t)(n * 4 + h) * G::CHUNK);
             load_words<2 * G::UNIT_GROUPS>(ks[i], p + G::K_SCALES + 2 * u * G::UNIT_GROUPS,
                                            (uint32_t)(2 * n * G::GROUPS));
@@ -61,23 +63,22 @@ template <int BITS, int D> struct Raw {
         const int operand = wave * S::V_ITEMS, pair = operand / (D / 16), u = operand % (D / 16) / G::COLUMN;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const uint8_t *p = place(2 * pair + i, v_valid[i]);
+            const uint8_t *p = place(2 * pair + i, 30 + i);
             load_words<G::CHUNK>(v[i], p + G::V_CODES + u * 64 * G::CHUNK, (uint32_t)(h * 16 + n) * G::CHUNK);
             load_words<8>(vs[i], p + G::V_SCALES + 8 * u * G::UNIT_GROUPS,
                           (uint32_t)(8 * (h * G::GROUPS + n * G::COLUMN / 32)));
-            v_first[i] = 16 * (first_tile + 2 * pair + i) + 4 * h;
         }
     }
 
-    // `edge`: some token of the step may be unwritten or on no page.
-    __device__ __forceinline__ void decode(uint4 (*kb)[64], uint4 (*vb)[64], int from, int to, bool edge, int wave,
-                                           int lane) {
+    // To LDS, V's scales of tokens outside [from, to) or on no page as zeros.
+    __device__ __forceinline__ void decode(uint4 (*kb)[64], uint4 (*vb)[64], int step, int from, int to, int wave,
+                                           int lane) const {
 #pragma unroll
         for (int i = 0; i < S::K_ITEMS; ++i) {
             const int item = wave * S::K_ITEMS + i, tile = item / G::UNITS, u = item % G::UNITS;
 #pragma unroll
             for (int g = 0; g < G::UNIT_GROUPS; ++g) {
-                const half2v s = as_half2(ks[i][g >> 1]), d = {s[g & 1], s[g & 1]}, b = bias_of<BITS>(d);
+                const half2v d = both(ks[i][g >> 1], g & 1), b = bias_of<BITS>(d);
                 Operand o;
                 if constexpr (BITS == 4) o = decode_k4(k[i][g], d, b);
                 else o = decode_k8(k[i][2 * g], k[i][2 * g + 1], d, b);
@@ -85,13 +86,15 @@ template <int BITS, int D> struct Raw {
             }
         }
         const int operand = wave * S::V_ITEMS, j0 = operand % G::COLUMN;
+        const int first = S::TOKENS * step, v_first = first + 32 * (operand / (D / 16)) + 4 * (lane >> 4);
+        const bool edge = first < from || first + S::TOKENS > to || there >> 30 != 3;
         uint32_t out[4][S::V_ITEMS];
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
             const int i = x >> 1, pair = x & 1;
             uint32_t scales = vs[i][pair];
             if (edge) {
-                const int t = v_first[i] + 2 * pair, end = v_valid[i] ? to : 0;
+                const int t = v_first + 16 * i + 2 * pair, end = (there >> (30 + i) & 1u) ? to : 0;
                 uint32_t mask = 0;
                 if (t >= from && t < end) mask |= 0xffffu;
                 if (t + 1 >= from && t + 1 < end) mask |= 0xffff0000u;
@@ -153,12 +156,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_prompt_kernel(CacheVi
 
     Raw<BITS, D> raw;
     const auto decode = [&](int step, int buffer) {
-        const int first = S::TOKENS * step;
 #pragma unroll
         for (int i = 0; i < S::K_ITEMS; ++i)
-            if (lane == 0) valid[buffer][(wave * S::K_ITEMS + i) / G::UNITS] = raw.k_valid[i];
-        const bool edge = first < s.from || first + S::TOKENS > s.to || !raw.v_valid[0] || !raw.v_valid[1];
-        raw.decode(kb[buffer], vb[buffer], s.from, s.to, edge, wave, lane);
+            if (lane == 0) valid[buffer][(wave * S::K_ITEMS + i) / G::UNITS] = (int)(raw.there >> i & 1u);
+        raw.decode(kb[buffer], vb[buffer], step, s.from, s.to, wave, lane);
     };
     if (s.low < s.high) raw.load(c, table, head, s.low, s.to, wave, n, h);
     rows.prepare(queries);

@@ -35,6 +35,13 @@ struct Operand {  // 8 f16 of one lane
     __device__ __forceinline__ half4 low() const { return __builtin_shufflevector(get(), get(), 0, 1, 2, 3); }
 };
 
+// A pair of one of a pair's halves. (No subscript that a loop makes: it kept whole
+// structs in memory.)
+__device__ __forceinline__ half2v both(uint32_t pair, int which) {
+    const half2v s = as_half2(pair);
+    return which ? half2v{s[1], s[1]} : half2v{s[0], s[0]};
+}
+
 // (x & mask) | bits as the one instruction it is: it takes one constant from a
 // scalar register, so the compiler, left to itself, keeps both there and issues two.
 __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
@@ -140,10 +147,7 @@ template <int BITS, int D> struct Tile {
         }
         load_words<2 * G::GROUPS>(ks, tile + G::K_SCALES, (uint32_t)(2 * n * G::GROUPS));
     }
-    __device__ __forceinline__ half2v k_scale(int g) const {
-        const half2v s = as_half2(ks[g >> 1]);
-        return half2v{s[g & 1], s[g & 1]};
-    }
+    __device__ __forceinline__ half2v k_scale(int g) const { return both(ks[g >> 1], g & 1); }
     __device__ __forceinline__ Operand k_operand(int u, int gi, half2v d) const {
         const half2v b = bias_of<BITS>(d);
         if constexpr (BITS == 4) return decode_k4(k[u][gi], d, b);
@@ -301,7 +305,14 @@ template <int BITS, int D, int RT, bool F32> struct Rows {
             top[t] = LOWEST, sum[t] = 0.0f;
 #pragma unroll
             for (int j = 0; j < TILES_O; ++j) o[t][j] = floatx4{0, 0, 0, 0};
-            if constexpr (F32) {
+            if constexpr (!F32) {
+                // waited for here: left to their first use, in the loop, they would be waited for
+                // in every turn of it, and with them the loads on their way
+#pragma unroll
+                for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) asm volatile("" : "+v"(q[0][t][g].w[e]));
+            } else {
                 float most = 0.0f;
 #pragma unroll
                 for (int g = 0; g < GROUPS; ++g)
