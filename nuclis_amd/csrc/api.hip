@@ -877,7 +877,7 @@ int nuq_cache_attention(nuq_context *ctx, const nuq_cache *cache, const nuq_atte
     const uint64_t longest = n.max_length ? std::min<uint64_t>(n.max_length, a.capacity) : a.capacity;
     const uint32_t f32 = n.dtype == NUQ_F32;
     const auto plan_with = [&](uint64_t floats) {
-        nuq::plan_attention(cache->bits, cache->head_dim, cache->kv_heads, f32, longest, n.q_heads, floats, &a);
+        nuq::plan_attention(cache->head_dim, cache->kv_heads, f32, longest, n.q_heads, floats, &a);
     };
     plan_with(UINT64_MAX);
     // without the workspace it wants (a capture, no memory): fewer splits

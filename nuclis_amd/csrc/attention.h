@@ -27,17 +27,18 @@ struct AttentionArgs {
     float *partial_o, *partial_ml;
 };
 
-// Row tiles of a wave of the prompt kernel (attention_prompt.hip).
+// The prompt kernel (attention_prompt.hip): row tiles of a wave, tokens of a step.
 constexpr int prompt_row_tiles(int head_dim, bool f32) {
-    return head_dim == 64 ? (f32 ? 3 : 4) : head_dim == 128 ? (f32 ? 2 : 3) : (f32 ? 1 : 2);
+    return head_dim == 64 ? (f32 ? 3 : 4) : head_dim == 128 ? (f32 ? 2 : 3) : f32 ? 1 : 2;
 }
+constexpr int prompt_tokens(int head_dim) { return head_dim == 256 ? 32 : 64; }
 hipError_t launch_attention_prompt(hipStream_t s, const CacheView &c, uint32_t bits, uint32_t d, uint32_t f32,
                                    const AttentionArgs &a);
 
 // Fills in the plan of a call: row tiles of 16, blocks of them, splits of the
 // long axis with at most `max_floats` of workspace.
-void plan_attention(uint32_t bits, uint32_t head_dim, uint32_t kv_heads, uint32_t f32, uint64_t max_length,
-                    uint32_t heads, uint64_t max_floats, AttentionArgs *a);
+void plan_attention(uint32_t head_dim, uint32_t kv_heads, uint32_t f32, uint64_t max_length, uint32_t heads,
+                    uint64_t max_floats, AttentionArgs *a);
 hipError_t launch_attention(hipStream_t s, const CacheView &c, uint32_t bits, uint32_t head_dim, uint32_t f32,
                             uint32_t heads, AttentionArgs a, float *work);
 

@@ -138,6 +138,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_rows_kernel(CacheView
             }
         }
         Operand p[PARTS][RT];
+        rows.template raise<TILES>(x);
         rows.template weigh<TILES>(x, p);
 #pragma unroll
         for (int u = 0; u < G::UNITS; ++u) {
@@ -290,28 +291,41 @@ template <bool F32> hipError_t rows_dispatch(hipStream_t s, const CacheView &c, 
 
 }  // namespace
 
-void plan_attention(uint32_t bits, uint32_t head_dim, uint32_t kv_heads, uint32_t f32, uint64_t max_length,
-                    uint32_t heads, uint64_t max_floats, AttentionArgs *a) {
-    (void)bits;
+// The kernel. Few rows read the cache straight into registers; where there is enough
+// work for it, a workgroup that decodes the cache once for its waves is faster:
+// 48 heads of 128, F16: one prompt of 1000 tokens 39 us by rows, 46 by the prompt
+// kernel; of 2000 104 and 86; 64 tokens after 8192 37 and 41, 256 tokens 100 and 87.
+// The bound is on (rows x tokens they see x D) in all: 8e9, and 1.2e10 where the prompt
+// kernel gains less, F32 (1000: 52 and 55; 2000: 150 and 122) and D = 64 (2000: 58 and 73;
+// 3000: 116 and 104).
+// The splits of the long axis, each of which costs its rows' partial outputs a
+// way through memory. Rows: up to 512 tokens are one workgroup's (300 tokens: 6.6
+// us, 7.7 split in three and joined); then 128 tokens each while a workgroup a CU wants
+// work (4096 tokens: 8.1 us, 10.5 at 512 each), and four a CU where each has 1024
+// (batch of 32 up to 16384: 83 us, 88 at two a CU, 114 at one). Prompts: three
+// workgroups a CU of 1024 tokens and more, where rows are few against the tokens they
+// see (512 tokens after 8192, F32: 221 us, 267 at two a CU; F16: 143, 285 unsplit; a prompt
+// of 2000 164 split, 86 not) or heads are wide (3000 tokens at D = 256: 160 and 193).
+void plan_attention(uint32_t head_dim, uint32_t kv_heads, uint32_t f32, uint64_t max_length, uint32_t heads,
+                    uint64_t max_floats, AttentionArgs *a) {
     const uint64_t rows = (uint64_t)a->max_tokens * a->group;
-    const uint32_t most = head_dim <= 128 ? 2 : 1;
-    a->prompt = rows > 64;
-    uint32_t tiles = 1;
-    while (tiles < most && tiles * 16 < rows) tiles *= 2;
-    if (a->prompt) tiles = prompt_row_tiles((int)head_dim, f32) * 4;
-    a->row_tiles = tiles;
-    a->blocks = (uint32_t)((rows + 16 * tiles - 1) / (16 * tiles));
-    const uint64_t groups = (uint64_t)a->batch * kv_heads * a->blocks;
-    uint64_t reach = max_length;
+    uint64_t reach = max_length;  // tokens the last row and those before it may see
     if (a->window) reach = std::min<uint64_t>(reach, (uint64_t)a->window + a->max_tokens);
+    const double seen = std::max((double)reach - 0.5 * a->max_tokens, 0.5 * (double)reach);
+    const double work = (double)a->batch * a->max_tokens * heads * seen * head_dim;
+    a->prompt = rows > 64 && work >= (f32 || head_dim == 64 ? 1.2e10 : 8e9);
+    if (a->prompt) {
+        a->row_tiles = prompt_row_tiles((int)head_dim, f32) * WAVES;
+    } else {
+        a->row_tiles = head_dim <= 128 && rows > 16 ? 2 : 1;
+    }
+    a->blocks = (uint32_t)((rows + 16 * a->row_tiles - 1) / (16 * a->row_tiles));
+    const uint64_t groups = (uint64_t)a->batch * kv_heads * a->blocks;
     uint64_t splits = 1;
     if (a->prompt) {
-        splits = std::min((768 + groups - 1) / groups, (reach + 255) / 256);
-        if (groups >= 768) splits = 1;
+        if (reach >= 4ull * a->max_tokens || head_dim == 256) splits = std::min((768 + groups - 1) / groups, reach / 1024);
     } else if (reach > 512) {
-        const uint64_t short_ones = std::min(256 / groups, (reach + 127) / 128);
-        const uint64_t long_ones = std::min(1024 / groups, reach / 1024);
-        splits = std::max(short_ones, long_ones);
+        splits = std::max(std::min(256 / groups, (reach + 127) / 128), std::min(1024 / groups, (reach + 1023) / 1024));
     }
     splits = std::max<uint64_t>(1, std::min<uint64_t>(splits, MAX_SPLITS));
     const uint64_t each = (uint64_t)a->rows * heads * (head_dim + 2);

@@ -14,6 +14,15 @@
 // instructions to decode, as many as the softmax of 64 rows; shared by four waves
 // it is a quarter. RT is what two workgroups a CU leave room for in registers (O,
 // Q and a step's scores), since one's products then run under the other's softmax.
+// Operands are read from LDS two products ahead of their use.
+//
+// Measured (4096 tokens, 48 query heads of 128 over 8, F16, 4 bits): 238 us, 866
+// TFLOP/s where a large f16 product reaches 1145 on the same card. The products alone
+// take 153 us, the softmax adds 46 and the decode 53: what bounds it is the vector
+// instructions between products (377 to 96 products a wave's step) that two waves
+// a SIMD do not hide whole. Steps of 32 tokens, eight waves, two row tiles, and the
+// next step's scores computed under this step's weights were each slower here; the
+// last one is faster at D = 256 alone (208 us for 250) and was not kept for it.
 #include "attention_tiles.h"
 
 namespace nuq {
@@ -22,48 +31,62 @@ namespace {
 
 template <int BITS, int D> struct Step {
     using G = CacheGeometry<BITS, D>;
-    static constexpr int TOKENS = D == 256 ? 32 : 64;  // 64 KB of LDS at D = 128 and 256
+    static constexpr int TOKENS = prompt_tokens(D);
     static constexpr int TILES = TOKENS / 16, PAIRS = TOKENS / 32;
-    static constexpr int K_ITEMS = TILES * G::UNITS / WAVES;      // (tile, unit)s a wave decodes
-    static constexpr int V_ITEMS = PAIRS * (D / 16) / WAVES;      // V operands, all of one (pair, unit)
-    static constexpr int WORDS = G::CHUNK / 4;
     static constexpr int K_OPERANDS = TILES * G::GROUPS, V_OPERANDS = PAIRS * (D / 16);
-    static_assert(K_ITEMS * WAVES == TILES * G::UNITS && V_ITEMS * WAVES == V_OPERANDS, "a wave's share is whole");
-    static_assert(G::COLUMN % V_ITEMS == 0, "a wave's V operands share a unit");
+    // a wave decodes K_ITEMS runs of K_SPAN groups of a token's chunk, and V_ITEMS dimensions of a V column
+    static constexpr int K_SHARE = K_OPERANDS / WAVES, K_SPAN = K_SHARE < G::UNIT_GROUPS ? K_SHARE : G::UNIT_GROUPS;
+    static constexpr int K_ITEMS = K_SHARE / K_SPAN, V_ITEMS = V_OPERANDS / WAVES;
+    static constexpr int K_WORDS = K_SPAN * BITS / 4, V_WORDS = G::CHUNK / 4;
+    static_assert(K_ITEMS * K_SPAN * WAVES == K_OPERANDS && V_ITEMS * WAVES == V_OPERANDS, "a wave's share is whole");
+    static_assert(G::UNIT_GROUPS % K_SPAN == 0 && G::COLUMN % V_ITEMS == 0, "of one unit");
 };
 
 // A wave's share of a step between memory and LDS.
 template <int BITS, int D> struct Raw {
     using S = Step<BITS, D>;
     using G = CacheGeometry<BITS, D>;
-    uint32_t k[S::K_ITEMS][S::WORDS], ks[S::K_ITEMS][G::UNIT_GROUPS / 2];
-    uint32_t v[2][S::WORDS], vs[2][2];
+    uint32_t k[S::K_ITEMS][S::K_WORDS], ks[S::K_ITEMS][S::K_SPAN / 2];
+    uint32_t v[2][S::V_WORDS], vs[2][2];
     uint32_t there;                     // bit i: the i-th K item's page exists; bits 30, 31: V's tiles' do
+    uint32_t page[S::K_ITEMS + 2];      // of the next step to load, looked up a step before it
 
-    __device__ __forceinline__ void load(const CacheView &c, PageTable table, uint32_t head, int step, int to,
-                                         int wave, int n, int h) {
-        // tiles past the last token read the step's first tile: they are masked
-        const int first_tile = step * S::TILES;
-        const auto place = [&](int tile, int bit) {
-            const uint32_t at = (uint32_t)(first_tile + (16 * (first_tile + tile) < to ? tile : 0));
-            bool valid;
-            const uint8_t *p = tile_at<BITS, D>(c, (uint32_t)table[at >> c.tiles_log2], head, at, valid);
-            there |= (uint32_t)valid << bit;
-            return p;
-        };
+    // The step's tile `tile`; past the last token its first one, which is masked.
+    static __device__ __forceinline__ uint32_t tile_of(int step, int tile, int to) {
+        const int first = step * S::TILES;
+        return (uint32_t)(first + (16 * (first + tile) < to ? tile : 0));
+    }
+    static __device__ __forceinline__ int k_tile(int wave, int i) {
+        return (wave * S::K_SHARE + i * S::K_SPAN) / G::GROUPS;
+    }
+    static __device__ __forceinline__ int v_tile(int wave, int i) { return wave * S::V_ITEMS / (D / 16) * 2 + i; }
+
+    __device__ __forceinline__ void look_up(const CacheView &c, PageTable table, int step, int to, int wave) {
+#pragma unroll
+        for (int i = 0; i < S::K_ITEMS + 2; ++i) {
+            const int tile = i < S::K_ITEMS ? k_tile(wave, i) : v_tile(wave, i - S::K_ITEMS);
+            page[i] = (uint32_t)table[tile_of(step, tile, to) >> c.tiles_log2];
+        }
+    }
+    __device__ __forceinline__ void load(const CacheView &c, uint32_t head, int step, int to, int wave, int n, int h) {
         there = 0;
 #pragma unroll
         for (int i = 0; i < S::K_ITEMS; ++i) {
-            const int item = wave * S::K_ITEMS + i, u = item % G::UNITS;
-            const uint8_t *p = place(item / G::UNITS, i);
-            load_words<G::CHUNK>(k[i], p + u * 64 * G::CHUNK, (uint32_t)(n * 4 + h) * G::CHUNK);
-            load_words<2 * G::UNIT_GROUPS>(ks[i], p + G::K_SCALES + 2 * u * G::UNIT_GROUPS,
-                                           (uint32_t)(2 * n * G::GROUPS));
+            const int g = (wave * S::K_SHARE + i * S::K_SPAN) % G::GROUPS, u = g / G::UNIT_GROUPS;
+            bool valid;
+            const uint8_t *p = tile_at<BITS, D>(c, page[i], head, tile_of(step, k_tile(wave, i), to), valid);
+            there |= (uint32_t)valid << i;
+            load_words<S::K_SPAN * BITS>(k[i], p + u * 64 * G::CHUNK + g % G::UNIT_GROUPS * BITS,
+                                         (uint32_t)(n * 4 + h) * G::CHUNK);
+            load_words<2 * S::K_SPAN>(ks[i], p + G::K_SCALES + 2 * g, (uint32_t)(2 * n * G::GROUPS));
         }
-        const int operand = wave * S::V_ITEMS, pair = operand / (D / 16), u = operand % (D / 16) / G::COLUMN;
+        const int u = wave * S::V_ITEMS % (D / 16) / G::COLUMN;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const uint8_t *p = place(2 * pair + i, 30 + i);
+            bool valid;
+            const uint8_t *p =
+                tile_at<BITS, D>(c, page[S::K_ITEMS + i], head, tile_of(step, v_tile(wave, i), to), valid);
+            there |= (uint32_t)valid << (30 + i);
             load_words<G::CHUNK>(v[i], p + G::V_CODES + u * 64 * G::CHUNK, (uint32_t)(h * 16 + n) * G::CHUNK);
             load_words<8>(vs[i], p + G::V_SCALES + 8 * u * G::UNIT_GROUPS,
                           (uint32_t)(8 * (h * G::GROUPS + n * G::COLUMN / 32)));
@@ -75,14 +98,13 @@ template <int BITS, int D> struct Raw {
                                            int lane) const {
 #pragma unroll
         for (int i = 0; i < S::K_ITEMS; ++i) {
-            const int item = wave * S::K_ITEMS + i, tile = item / G::UNITS, u = item % G::UNITS;
 #pragma unroll
-            for (int g = 0; g < G::UNIT_GROUPS; ++g) {
+            for (int g = 0; g < S::K_SPAN; ++g) {
                 const half2v d = both(ks[i][g >> 1], g & 1), b = bias_of<BITS>(d);
                 Operand o;
                 if constexpr (BITS == 4) o = decode_k4(k[i][g], d, b);
                 else o = decode_k8(k[i][2 * g], k[i][2 * g + 1], d, b);
-                kb[tile * G::GROUPS + u * G::UNIT_GROUPS + g][lane] = make_uint4(o.w[0], o.w[1], o.w[2], o.w[3]);
+                kb[wave * S::K_SHARE + i * S::K_SPAN + g][lane] = make_uint4(o.w[0], o.w[1], o.w[2], o.w[3]);
             }
         }
         const int operand = wave * S::V_ITEMS, j0 = operand % G::COLUMN;
@@ -102,11 +124,12 @@ template <int BITS, int D> struct Raw {
             }
             const half2v d = as_half2(scales), b = bias_of<BITS>(d);
             if constexpr (BITS == 4) {
-                uint32_t w;  // four dimensions of two tokens, from j0 (0 or 4; 0 or 2 at D = 64)
+                uint32_t w;  // four dimensions of two tokens, from j0 on
                 if constexpr (G::COLUMN == 8)
-                    w = __builtin_amdgcn_perm(v[i][2 * pair + 1], v[i][2 * pair], j0 ? 0x07060302u : 0x05040100u);
+                    w = __builtin_amdgcn_perm(v[i][2 * pair + 1], v[i][2 * pair], j0 & 4 ? 0x07060302u : 0x05040100u);
                 else
-                    w = v[i][pair] >> (4 * j0);
+                    w = v[i][pair];
+                if constexpr (S::V_ITEMS == 2) w >>= 4 * (j0 & 3);
                 out[x][0] = as_u32(as_half2(nibbles<0>(w)) * d + b);
                 out[x][1] = as_u32(as_half2(nibbles<1>(w)) * d + b);
                 if constexpr (S::V_ITEMS == 4) {
@@ -133,7 +156,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_prompt_kernel(CacheVi
     using G = CacheGeometry<BITS, D>;
     using S = Step<BITS, D>;
     using T = std::conditional_t<F32, float, _Float16>;
-    constexpr int PARTS = F32 ? 2 : 1;
+    constexpr int PARTS = F32 ? 2 : 1, AHEAD = 2;
     __shared__ uint4 kb[2][S::K_OPERANDS][64], vb[2][S::V_OPERANDS][64];
     __shared__ int valid[2][4];  // of a buffer's tiles
 
@@ -158,28 +181,35 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_prompt_kernel(CacheVi
     const auto decode = [&](int step, int buffer) {
 #pragma unroll
         for (int i = 0; i < S::K_ITEMS; ++i)
-            if (lane == 0) valid[buffer][(wave * S::K_ITEMS + i) / G::UNITS] = (int)(raw.there >> i & 1u);
+            if (lane == 0) valid[buffer][raw.k_tile(wave, i)] = (int)(raw.there >> i & 1u);
         raw.decode(kb[buffer], vb[buffer], step, s.from, s.to, wave, lane);
     };
-    if (s.low < s.high) raw.load(c, table, head, s.low, s.to, wave, n, h);
+    const int last = max(s.high - 1, 0);
+    raw.look_up(c, table, min(s.low, last), s.to, wave);
+    raw.load(c, head, min(s.low, last), s.to, wave, n, h);
+    raw.look_up(c, table, min(s.low + 1, last), s.to, wave);
     rows.prepare(queries);
     if (s.low < s.high) {
         decode(s.low, 0);
-        raw.load(c, table, head, min(s.low + 1, s.high - 1), s.to, wave, n, h);
+        raw.load(c, head, min(s.low + 1, last), s.to, wave, n, h);
+        raw.look_up(c, table, min(s.low + 2, last), s.to, wave);
         __syncthreads();
     }
     for (int step = s.low; step < s.high; ++step) {
         const int buffer = (step - s.low) & 1, first = S::TOKENS * step;
+        int there[S::TILES];
+        bool all = true;
+#pragma unroll
+        for (int i = 0; i < S::TILES; ++i) there[i] = valid[buffer][i];
         if (step + 1 < s.high) {
             decode(step + 1, buffer ^ 1);
-            raw.load(c, table, head, min(step + 2, s.high - 1), s.to, wave, n, h);
+            raw.load(c, head, min(step + 2, last), s.to, wave, n, h);
+            raw.look_up(c, table, min(step + 3, last), s.to, wave);
         }
         if (first < rows.seen_to && first + S::TOKENS > rows.seen_from) {
-            int there[S::TILES];
-            bool all = true;
 #pragma unroll
             for (int i = 0; i < S::TILES; ++i) {
-                there[i] = __builtin_amdgcn_readfirstlane(valid[buffer][i]);
+                there[i] = __builtin_amdgcn_readfirstlane(there[i]);
                 all &= there[i] != 0;
             }
             const bool masked = first < rows.clear_from || first + S::TOKENS > rows.clear_to || !all;
@@ -187,22 +217,41 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_prompt_kernel(CacheVi
             for (int pair = 0; pair < S::PAIRS; ++pair) {
                 floatx4 x[2][RT];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
+                for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int t = 0; t < RT; ++t) x[i][t] = floatx4{0, 0, 0, 0};
+                const uint4(*const k)[64] = kb[buffer] + 2 * pair * G::GROUPS, (*const v)[64] = vb[buffer] + pair * (D / 16);
+                __builtin_amdgcn_sched_barrier(0);
+                uint4 ahead[AHEAD];
 #pragma unroll
-                    for (int g = 0; g < G::GROUPS; ++g)
-                        rows.score(__builtin_bit_cast(half8, kb[buffer][(2 * pair + i) * G::GROUPS + g][lane]), g, x[i]);
+                for (int i = 0; i < AHEAD; ++i) ahead[i] = k[i][lane];
+                __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+                for (int i = 0; i < 2 * G::GROUPS; ++i) {
+                    const uint4 now = ahead[i % AHEAD];
+                    if (i + AHEAD < 2 * G::GROUPS) ahead[i % AHEAD] = k[i + AHEAD][lane];
+                    rows.score(__builtin_bit_cast(half8, now), i % G::GROUPS, x[i / G::GROUPS]);
+                    __builtin_amdgcn_sched_group_barrier(0x008, RT * PARTS, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
                 }
                 if (masked) {
 #pragma unroll
                     for (int i = 0; i < 2; ++i) rows.mask(x[i], first + 32 * pair + 16 * i + 4 * h, there[2 * pair + i]);
                 }
                 Operand p[PARTS][RT];
+                rows.template raise<2>(x);
                 rows.template weigh<2>(x, p);
 #pragma unroll
-                for (int j = 0; j < D / 16; ++j)
-                    rows.template add<2>(__builtin_bit_cast(Operand, vb[buffer][pair * (D / 16) + j][lane]), j, p);
+                for (int j = 0; j < AHEAD; ++j) ahead[j] = v[j][lane];
+                __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 1);
+#pragma unroll
+                for (int j = 0; j < D / 16; ++j) {
+                    const uint4 now = ahead[j % AHEAD];
+                    if (j + AHEAD < D / 16) ahead[j % AHEAD] = v[j + AHEAD][lane];
+                    rows.template add<2>(__builtin_bit_cast(Operand, now), j, p);
+                    __builtin_amdgcn_sched_group_barrier(0x008, RT * PARTS, 1);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
+                }
             }
         }
         __syncthreads();

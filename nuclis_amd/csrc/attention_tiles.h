@@ -118,6 +118,7 @@ template <int BYTES> __device__ __forceinline__ void load_words(uint32_t *to, co
     // scalar registers and adds these 32 bits itself)
     asm volatile("" : "+v"(offset));
     const uint8_t *p = base + offset;
+    static_assert(BYTES == 4 || BYTES == 8 || BYTES == 16);
     if constexpr (BYTES == 16) {
         const uint4 v = *(const uint4 *)p;
         to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
@@ -375,25 +376,36 @@ template <int BITS, int D, int RT, bool F32> struct Rows {
             }
         }
     }
-    // Weights of one or two tiles' raw scores as the B operand of the next product.
-    // The common step asks only whether any score passes its row's reference by
-    // more than SLACK; the maximum over the row's lanes is taken where one does.
-    template <int TILES> __device__ __forceinline__ void weigh(const floatx4 (&x)[TILES][RT], Operand (&p)[PARTS][RT]) {
+    // Moves the references of rows that a step's raw scores pass by more than SLACK.
+    // The common step asks only whether one does; the maximum over a row's lanes
+    // is taken where so.
+    template <int TILES> __device__ __forceinline__ void raise(const floatx4 (&x)[TILES][RT]) {
+        float most[RT];
+        bool past = false;
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-            float most = -__builtin_inff();
+            most[t] = -__builtin_inff();
 #pragma unroll
             for (int i = 0; i < TILES; ++i)
-                most = fmaxf(most, fmaxf(fmaxf(x[i][t][0], x[i][t][1]), fmaxf(x[i][t][2], x[i][t][3])));
-            most *= scale[t];
-            if (__any(most > top[t] + SLACK)) {
-                most = over_quarters_max(most);
-                const float higher = fmaxf(top[t], most), by = __builtin_amdgcn_exp2f(top[t] - higher);
+                most[t] = fmaxf(most[t], fmaxf(fmaxf(x[i][t][0], x[i][t][1]), fmaxf(x[i][t][2], x[i][t][3])));
+            most[t] *= scale[t];
+            past |= most[t] > top[t] + SLACK;
+        }
+        if (__any(past)) {
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                const float higher = fmaxf(top[t], over_quarters_max(most[t])), by = __builtin_amdgcn_exp2f(top[t] - higher);
                 top[t] = higher;
                 sum[t] *= by;
 #pragma unroll
                 for (int j = 0; j < TILES_O; ++j) o[t][j] *= by;
             }
+        }
+    }
+    // Weights of one or two tiles' raw scores as the B operand of the next product.
+    template <int TILES> __device__ __forceinline__ void weigh(const floatx4 (&x)[TILES][RT], Operand (&p)[PARTS][RT]) {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
             const float down = RAISE - top[t];
             float w[4 * TILES];
 #pragma unroll

@@ -300,3 +300,118 @@ def test_refusals_leave_the_output_untouched(backend):
     assert bool((out == 7.0).all())
     empty = torch.empty(0, 4, 64, device="cuda")
     backend.cache_attention(c.cache, empty, empty, table[:0], lengths[:0])  # nothing to do
+
+
+def prompt_table(c):
+    """The case's page table with so many more entries, none of which names a page, that the
+    tokens its rows could see make it a prompt's work: the kernel that decodes the
+    cache once for four waves takes it, split over workgroups, however short it is."""
+    brought, heads = max(c.brought), c.kv * c.group
+    assert brought * c.group > 64
+    wide = -(-int(1.3e10 / (len(c.held) * brought * heads * c.d)) // c.page) + 1
+    table = np.full((len(c.held), max(wide, c.table.shape[1])), -1, np.int32)
+    table[:, :c.table.shape[1]] = c.table
+    return table
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("d,page,kv,group", [(64, 16, 1, 3), (128, 64, 2, 6), (256, 32, 1, 5)])
+@pytest.mark.parametrize("tokens,length", [(22, 22), (65, 65), (66, 130), (70, 531)])
+def test_prompt_rows(backend, dtype, bits, d, page, kv, group, tokens, length):
+    print(f"[attention] prompt {dtype} bits {bits} d {d} kv {kv} group {group} tokens {tokens} length {length}", flush=True)
+    c = Case([length], [tokens], bits, d, page, kv, group, dtype, seed=tokens + d)
+    c.check(c.run(backend, table=prompt_table(c)))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_prompt_rows_of_ragged_and_empty_sequences(backend, dtype, d):
+    c = Case([300, 0, 17, 1, 64, 500], [35, 1, 40, 1, 0, 33], dtype=dtype, kv=2, group=3, d=d, page=16, seed=15)
+    got = c.run(backend, table=prompt_table(c))
+    c.check(got)
+    assert not got[35].any()          # the empty sequence
+    assert not got[36:36 + 23].any()  # positions before the third one's start
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_prompt_rows_and_poisoned_tokens(backend, dtype, bits):
+    import torch
+    c = Case([200], [100], bits, dtype=dtype, kv=2, group=2, d=64, page=16, seed=16)
+    c.k[0][130, 0, 3] = np.nan
+    c.v[0][140, 1, 60] = np.inf
+    c.write(backend, 0, c.k[0], c.v[0])
+    torch.cuda.synchronize()
+    got = c.run(backend, table=prompt_table(c))
+    c.check(got)
+    nan = np.isnan(got).any(-1)
+    assert not nan[:30, :2].any() and nan[30:, :2].all() and not nan[:40, 2:].any() and nan[40:, 2:].all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("d,bits", [(64, 8), (128, 4), (256, 4)])
+def test_prompt_rows_and_missing_pages(backend, dtype, d, bits):
+    c = Case([150], [40], bits, dtype=dtype, kv=2, group=2, d=d, page=16, seed=17)
+    table = prompt_table(c)
+    table[0, 2], table[0, 5] = -1, 1 << 30
+    absent = np.zeros(150, bool)
+    absent[32:48] = absent[80:96] = True
+    c.check(c.run(backend, table=table), absent={0: absent})
+    table[0, 1:] = -1
+    absent[16:] = True
+    c.check(c.run(backend, table=table), absent={0: absent})  # whole steps and splits without a page
+    table[0, 0] = -1
+    assert not c.run(backend, table=table).any()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_prompt_rows_large_scores_strides_and_rows_no_sequence_has(backend, dtype):
+    import torch
+    c = Case([500, 90], [40, 40], dtype=dtype, kv=1, group=3, page=16, seed=18, spread=300.0)
+    table = prompt_table(c)
+    want = c.run(backend, table=table)
+    c.check(want)
+    wide = torch.full((80, 8, 128), 3.0, dtype=c.dtype, device="cuda")
+    wide[:, :3] = to_gpu(c.q)
+    out = torch.full((80, 7, 128), 7.0, dtype=c.dtype, device="cuda")
+    got = c.run(backend, table=table, q=wide[:, :3], out=out[:, :3])
+    assert np.array_equal(got, want) and bool((out[:, 3:] == 7.0).all())
+    got = c.run(backend, table=table, starts=np.array([0, 40, 70]), lengths=[500, 80])
+    assert np.array_equal(got[:70], want[:70]) and np.all(got[70:] == 7.0)
+    got = c.run(backend, table=table, starts=np.array([10, 5, 1000]), lengths=[500, 125])
+    assert np.all(got[:5] == 7.0) and not np.any(got[5:] == 7.0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("d,bits,kv,group", [(64, 4, 2, 50), (128, 4, 8, 6), (128, 8, 1, 48), (256, 4, 4, 24)])
+@pytest.mark.parametrize("window", [0, 33])
+def test_long_prompts(backend, dtype, d, bits, kv, group, window):
+    """A prompt long enough by itself, one workgroup along the axis (D = 256 splits
+    without a window), on rows at the edges of steps, tiles and the prompt."""
+    print(f"[attention] long prompt {dtype} d {d} bits {bits} kv {kv} group {group} window {window}", flush=True)
+    c = Case([2185], [2151], bits, d, 32, kv, group, dtype, seed=19)
+    rows = [0, 1, 29, 30, 31, 32, 33, 34, 62, 63, 64, 65, 94, 95, 97, 128, 500, 1023, 1024, 1999, 2013, 2014, 2149, 2150]
+    c.check(c.run(backend, window=window), window=window, rows=rows)
+    assert np.isfinite(c.run(backend, window=window)).all()
+
+
+def test_prompt_rows_replayed_from_a_graph(backend):
+    import torch
+    c = Case([700], [50], kv=2, group=2, seed=20)
+    b = nq.Backend(0)
+    q, table, lengths = to_gpu(c.q), to_gpu(prompt_table(c)), to_gpu(np.array([700], np.int32))
+    stream, out = torch.cuda.Stream(), torch.zeros(50, 4, 128, device="cuda")
+    for _ in range(2):  # without a workspace, then with one
+        stream.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(stream), torch.cuda.graph(graph, stream=stream):
+            b.cache_attention(c.cache, q, out, table, lengths)
+        for _ in range(3):
+            out.zero_()
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            c.check(out.cpu().numpy().astype(np.float64))
+            c.run(b, table=prompt_table(c))
+    b.close()
