@@ -214,3 +214,52 @@ def test_writes_and_reads_replay_from_a_graph_on_another_stream(backend):
         want_k, want_v, _ = co.stored(bits, a, b)
         assert np.array_equal(kr.cpu().numpy().astype(np.float64), want_k)
         assert np.array_equal(vr.cpu().numpy().astype(np.float64), want_v)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_codes_at_the_edges_between_them(backend, bits):
+    """Inputs at (c + 1/2) d and one F32 step to either side of it, for every code and for
+    scales from the smallest an f16 holds to the largest kept: the codes are those of
+    IEEE's quotient, rounded to even."""
+    import torch
+    top, steps = (8, 8) if bits == 4 else (127, 4)
+    rng = np.random.default_rng(50)
+    mantissas = 1 + rng.integers(0, 1 << (steps - 1), 40) / (1 << (steps - 1))
+    scales = (mantissas * 2.0 ** rng.integers(-24, 11 if bits == 4 else 5, 40)).astype(np.float16).astype(np.float32)
+    groups = []
+    for d in scales:
+        middles = ((np.arange(-top, top) + 0.5) * np.float64(d)).astype(np.float32)
+        around = np.concatenate([np.nextafter(middles, np.float32(-np.inf)), middles, np.nextafter(middles, np.float32(np.inf))])
+        around = np.resize(around, -(-len(around) // 31) * 31).reshape(-1, 31)
+        # the extreme that makes the group's scale d
+        groups.append(np.concatenate([around, np.full((len(around), 1), -top * d if bits == 4 else top * d, np.float32)], 1))
+    x = np.concatenate(groups)
+    x = np.resize(x, (-(-len(x) // 4) * 4, 32)).reshape(-1, 1, 128)
+    cache = nq.KVCache(bits, -(-len(x) // 64), 64, 1, 128)
+    slots = torch.arange(len(x), device="cuda")
+    backend.cache_write(cache, to_gpu(x), to_gpu(-x), slots)
+    kr, vr = (torch.zeros(len(x), 1, 128, device="cuda") for _ in range(2))
+    backend.cache_read(cache, slots, kr, vr)
+    backend.sync()
+    want_k, want_v, _ = co.stored(bits, x, -x)
+    assert np.array_equal(kr.cpu().numpy().astype(np.float64), want_k)
+    assert np.array_equal(vr.cpu().numpy().astype(np.float64), want_v)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_the_largest_numbers_of_f32(backend, bits):
+    import torch
+    x = values(51, (40, 2, 64))
+    x[::3, 0] *= np.float32(3e37)
+    x[1, 1, ::5] = np.finfo(np.float32).max
+    x[2, 1, ::7] = -np.finfo(np.float32).max
+    x[5, 0] = np.float32(1e-40)
+    cache = nq.KVCache(bits, 3, 16, 2, 64)
+    slots = torch.arange(40, device="cuda")
+    backend.cache_write(cache, to_gpu(x), to_gpu(-x), slots)
+    kr, vr = (torch.zeros(40, 2, 64, device="cuda") for _ in range(2))
+    backend.cache_read(cache, slots, kr, vr)
+    backend.sync()
+    want_k, want_v, _ = co.stored(bits, x, -x)
+    assert np.array_equal(kr.cpu().numpy().astype(np.float64), want_k)
+    assert np.array_equal(vr.cpu().numpy().astype(np.float64), want_v)
