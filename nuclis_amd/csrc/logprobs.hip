@@ -17,9 +17,10 @@
 // waves' queues, cut by the last bound, are ranked by counting.
 //
 // Bound by the read of the logits: 1024 rows of 151936 F32 logits with five
-// alternatives take 118 us, 5.3 TB/s (without alternatives 115; as F16 69). The
-// next step's loads are on the way during a step's work. Each wave with a bound of
-// its own took 161 us: three times the steps looked at single logits.
+// alternatives take 107 us, 5.8 TB/s (without alternatives 103; as F16 67). The
+// next step's loads are on the way during a step's work, past the caches (118 us
+// with ordinary loads: nothing is read twice). Each wave with a bound of its own
+// took 161 us: three times the steps looked at single logits.
 // A row is split over workgroups where there are few rows, a step each at the
 // least; the splits' results go to the workspace for a second kernel. One row
 // takes 11 us with twenty alternatives, 64 rows 23 us: a split has a few steps and
@@ -31,6 +32,7 @@ namespace nuq {
 namespace {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float LOWEST = -3.402823466e38f, LOG2E = 1.44269504088896340736f;
 constexpr uint64_t PAD = ~0ull;  // after every key
@@ -206,12 +208,13 @@ __global__ void __launch_bounds__(THREADS) logprobs_kernel(LogprobArgs a) {
     const uint32_t full = before ? 1 : 0, full_end = (uint32_t)((before + (uint64_t)a.count) / V);
     // The next step's vectors are requested before this step's are worked on, from a
     // whole vector's place whatever theirs: no condition stands between the loads.
-    uint4 next[VECTORS] = {};
+    u32x4 next[VECTORS] = {};
     const auto request = [&](uint32_t base) {
 #pragma unroll
         for (int u = 0; u < VECTORS; ++u) {
             const uint32_t at = min(max(base + u * THREADS + tid, full), full_end - 1);
-            next[u] = *(const uint4 *)((const uint8_t *)x - before * (int)sizeof(T) + 16ull * at);
+            next[u] = __builtin_nontemporal_load(
+                (const u32x4 *)((const uint8_t *)x - before * (int)sizeof(T) + 16ull * at));
         }
     };
     if (full < full_end) request(split * a.span);
