@@ -882,8 +882,9 @@ int nuq_cache_attention(nuq_context *ctx, const nuq_cache *cache, const nuq_atte
     plan_with(UINT64_MAX);
     // without the workspace it wants (a capture, no memory): fewer splits
     if (!ensure_workspace(ctx, a.floats)) plan_with((uint64_t)ctx->split.tiles * 256 * 256);
+    // (splits are taken where there are few workgroups: the second kernel's are fewer still)
     if ((uint64_t)cache->kv_heads * a.splits * a.blocks * a.batch > 0x00ffffffull ||
-        (uint64_t)a.batch * a.max_tokens * n.q_heads > 0x00ffffffull)
+        (a.splits > 1 && (uint64_t)a.batch * a.max_tokens * n.q_heads > 0x00ffffffull))
         return fail(ctx, NUQ_INVALID_SHAPE, "too many query rows for one call");
     return hip_check(ctx,
                      nuq::launch_attention(ctx->stream, view, cache->bits, cache->head_dim, f32, n.q_heads, a,

@@ -31,6 +31,12 @@
 // Work split. The four waves of a workgroup take steps of 32 tokens in turn and
 // are merged in LDS; a long axis with few rows is split over workgroups, whose
 // partial (maximum, sum, output) go to the workspace for a second kernel.
+//
+// Measured (48 query heads of 128 over 8, 4 bits). One F32 token after 300 tokens:
+// 6.6 us, a chain of four trips to memory; after 32768: 13.7 us and 3.8 for the
+// second kernel (37.8 MB, 7.8 us at a copy's rate). 32 sequences of one F16 token up to
+// 16384: 69 and 4.7 us, 4.6 TB/s, with the vector units half busy. 4 x 8 F32 tokens up
+// to 8191 at 8 bits: 20.6 and 4.0 us, latency and the decode of two blocks of rows.
 #include "attention_tiles.h"
 
 #include <algorithm>
@@ -215,8 +221,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_rows_kernel(CacheView
 
 // Joins the splits of one (sequence, token, head) a workgroup: the first wave
 // turns the splits' maxima into weights, then D / 4 threads take a split, 1024 / D
-// splits at a time. (A split without a token has sum 0 and zeros. One wave walking 64 splits in order took 29 us after 32768 tokens,
-// one round of memory latency a split; this takes 3.9.)
+// splits at a time. (A split without a token has sum 0 and zeros. One wave walking 64
+// splits in order took 29 us after 32768 tokens, one round of memory latency a split;
+// this takes 3.8.)
 template <int D, bool F32>
 __global__ void __launch_bounds__(256) attention_join_kernel(AttentionArgs a, uint32_t heads) {
     using T = std::conditional_t<F32, float, _Float16>;
@@ -264,6 +271,50 @@ __global__ void __launch_bounds__(256) attention_join_kernel(AttentionArgs a, ui
     }
     const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
     store4((T *)a.out + row * a.out_stride + head * D + x4, x, inverse);
+}
+
+// The same where splits are few (up to 8): D / 4 threads take a (sequence, token, head) and
+// walk them, four on their way together. (2 x 1000 tokens of 16 heads of 256 in three splits: the
+// call takes 149 us, 160 with a workgroup each; 8 splits about even; 32 splits of one
+// token 18.6, 16.3 with a workgroup each.)
+template <int D, bool F32>
+__global__ void __launch_bounds__(256) attention_join_rows_kernel(AttentionArgs a, uint32_t heads, uint32_t items) {
+    using T = std::conditional_t<F32, float, _Float16>;
+    constexpr int ACROSS = D / 4, SIDE = 256 / ACROSS;
+    const uint32_t item = blockIdx.x * SIDE + threadIdx.x / ACROSS, x4 = 4 * (threadIdx.x % ACROSS);
+    if (item >= items) return;
+    const uint32_t head = item % heads, token = item / heads % a.max_tokens, b = item / heads / a.max_tokens;
+    int begin, tokens;
+    rows_of(a, b, begin, tokens);
+    if ((int)token >= tokens) return;
+    const uint64_t row = (uint64_t)begin + token, at = row * heads + head;
+    const float *ml = a.partial_ml + 2 * at * a.splits, *p = a.partial_o + at * a.splits * D + x4;
+    float4 x = make_float4(0, 0, 0, 0);
+    float top = LOWEST, sum = 0.0f;
+    constexpr uint32_t EACH = 4;  // splits on their way together
+    for (uint32_t first = 0; first < a.splits; first += EACH) {
+        float4 y[EACH];
+        float m[EACH], l[EACH];
+#pragma unroll
+        for (uint32_t j = 0; j < EACH; ++j) {
+            const uint32_t i = min(first + j, a.splits - 1);
+            y[j] = *(const float4 *)(p + (uint64_t)i * D);
+            m[j] = ml[2 * i], l[j] = ml[2 * i + 1];
+            if (first + j >= a.splits) l[j] = 0.0f;
+            if (l[j] == 0.0f) m[j] = LOWEST;
+        }
+        float above = top;
+#pragma unroll
+        for (uint32_t j = 0; j < EACH; ++j) above = fmaxf(above, m[j]);
+        const float by = __builtin_amdgcn_exp2f(top - above);
+        x.x *= by, x.y *= by, x.z *= by, x.w *= by, sum *= by, top = above;
+#pragma unroll
+        for (uint32_t j = 0; j < EACH; ++j) {
+            const float w = l[j] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m[j] - top);
+            x.x += w * y[j].x, x.y += w * y[j].y, x.z += w * y[j].z, x.w += w * y[j].w, sum += w * l[j];
+        }
+    }
+    store4((T *)a.out + row * a.out_stride + head * D + x4, x, sum == 0.0f ? 0.0f : 1.0f / sum);
 }
 
 template <int BITS, int D, int RT, bool F32>
@@ -344,11 +395,15 @@ hipError_t launch_attention(hipStream_t s, const CacheView &c, uint32_t bits, ui
                          : f32    ? rows_dispatch<true>(s, c, bits, head_dim, a)
                                   : rows_dispatch<false>(s, c, bits, head_dim, a);
     if (e != hipSuccess || a.splits == 1) return e;
-    const uint32_t grid = a.batch * a.max_tokens * heads;
-#define NUQ_CASE(D)                                                                                  \
-    if (head_dim == D) {                                                                             \
-        if (f32) attention_join_kernel<D, true><<<grid, 256, 0, s>>>(a, heads);                      \
-        else attention_join_kernel<D, false><<<grid, 256, 0, s>>>(a, heads);                         \
+    const uint32_t items = a.batch * a.max_tokens * heads;
+    const bool few_splits = a.splits <= 8;
+#define NUQ_CASE(D)                                                                                              \
+    if (head_dim == D) {                                                                                         \
+        const uint32_t grid = (items + 1024 / D - 1) / (1024 / D);                                                \
+        if (few_splits && f32) attention_join_rows_kernel<D, true><<<grid, 256, 0, s>>>(a, heads, items);                \
+        else if (few_splits) attention_join_rows_kernel<D, false><<<grid, 256, 0, s>>>(a, heads, items);                 \
+        else if (f32) attention_join_kernel<D, true><<<items, 256, 0, s>>>(a, heads);                            \
+        else attention_join_kernel<D, false><<<items, 256, 0, s>>>(a, heads);                                    \
     }
     NUQ_CASE(64) NUQ_CASE(128) NUQ_CASE(256)
 #undef NUQ_CASE

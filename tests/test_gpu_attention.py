@@ -415,3 +415,20 @@ def test_prompt_rows_replayed_from_a_graph(backend):
             c.check(out.cpu().numpy().astype(np.float64))
             c.run(b, table=prompt_table(c))
     b.close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("d,kv,group,lengths,tokens", [(64, 2, 5, [1900, 0, 3100], [3, 1, 2]), (128, 1, 3, [2500, 2499], [1, 1]),
+                                                       (256, 4, 2, [4100, 40], [5, 3]), (128, 8, 6, [3000] * 9, [2] * 9)])
+def test_few_and_many_splits_of_ragged_rows(backend, dtype, d, kv, group, lengths, tokens):
+    """Axes split by a few (bounds on the length that ask for 2 to 8) and by many, with splits that hold
+    nothing of the short sequences."""
+    c = Case(lengths, tokens, 4, d, 32, kv, group, dtype, seed=21)
+    for bound in (0, 200, 600, 1000, 2100):
+        c.check(c.run(backend, max_length=bound))
+
+
+def test_a_prompt_among_many_single_tokens(backend):
+    """One call for a long prompt and hundreds of sequences that bring a token each."""
+    c = Case([1000] + [5] * 399, [1000] + [1] * 399, d=64, kv=1, group=48, page=16, dtype="f16", seed=22)
+    c.check(c.run(backend), rows=[0, 1, 63, 64, 511, 998, 999])
