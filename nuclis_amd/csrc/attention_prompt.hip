@@ -21,8 +21,7 @@
 // take 153 us, the softmax adds 46 and the decode 53: what bounds it is the vector
 // instructions between products (377 to 96 products a wave's step) that two waves
 // a SIMD do not hide whole. Steps of 32 tokens, eight waves, two row tiles, and the
-// next step's scores computed under this step's weights were each slower here; the
-// last one is faster at D = 256 alone (208 us for 250) and was not kept for it.
+// next step's scores computed under this step's weights were each slower or equal.
 #include "attention_tiles.h"
 
 namespace nuq {
