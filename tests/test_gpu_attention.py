@@ -432,3 +432,27 @@ def test_a_prompt_among_many_single_tokens(backend):
     """One call for a long prompt and hundreds of sequences that bring a token each."""
     c = Case([1000] + [5] * 399, [1000] + [1] * 399, d=64, kv=1, group=48, page=16, dtype="f16", seed=22)
     c.check(c.run(backend), rows=[0, 1, 63, 64, 511, 998, 999])
+
+
+@pytest.mark.parametrize("tokens", [2, 70])
+def test_offsets_past_32_bits(backend, tokens):
+    """Pages beyond 4 GiB of a cache, and query and output rows beyond 2^32 bytes of their buffers,
+    give what the same tokens give near their starts, by rows and as a prompt."""
+    import torch
+    c = Case([131], [tokens], kv=8, group=1, page=64, dtype="f16", seed=23)
+    table = c.table if tokens < 64 else prompt_table(c)
+    want = c.run(backend, table=table)
+    c.check(want)
+    pages = (1 << 32) // (64 * 8 * 144) + 8
+    far = nq.KVCache(4, pages, 64, 8, 128)
+    page_bytes = 64 * 8 * 144
+    moved = np.where((table >= 0) & (table < c.cache.pages), table + pages - c.cache.pages, -1).astype(np.int32)
+    far.bytes[(pages - c.cache.pages) * page_bytes:] = c.cache.bytes
+    c.cache = far
+    assert np.array_equal(c.run(backend, table=moved), want)
+    stride = (1 << 32) // (2 * (tokens - 1)) // 8 * 8 + 1024
+    held = torch.empty(2, (tokens - 1) * stride + 1024, dtype=torch.float16, device="cuda")
+    q, out = (h.as_strided((tokens, 8, 128), (stride, 128, 1)) for h in held)
+    q.copy_(to_gpu(c.q))
+    out.fill_(7.0)
+    assert np.array_equal(c.run(backend, table=moved, q=q, out=out), want)

@@ -181,3 +181,24 @@ def test_refusals_leave_the_results_untouched(backend):
     backend.sync()
     assert bool((lp == 5).all()) and bool((entropy == 5).all()) and bool((ids == 5).all()) and bool((tops == 5).all())
     backend.logprobs(x[:0], targets[:0], lp[:0], entropy[:0])  # no rows: nothing to do
+
+
+def test_rows_past_32_bits_of_bytes(backend):
+    import torch
+    x = (3 * np.random.default_rng(60).standard_normal((3, 5001))).astype(np.float32)
+    stride = (1 << 30) + 3
+    held = torch.empty(2 * stride + 5001, device="cuda")
+    far = held.as_strided((3, 5001), (stride, 1))
+    far.copy_(to_gpu(x))
+    results = []
+    for logits in (to_gpu(x), far):
+        out = [torch.empty(3, device="cuda"), torch.empty(3, device="cuda"),
+               torch.empty(3, 7, dtype=torch.int32, device="cuda"), torch.empty(3, 7, device="cuda")]
+        backend.logprobs(logits, torch.tensor([1, 5000, 77], dtype=torch.int32, device="cuda"), *out)
+        backend.sync()
+        results.append([t.cpu().numpy() for t in out])
+    near, far_ones = results
+    order = np.argsort(-x, axis=1, kind="stable")[:, :7]
+    assert np.array_equal(near[2], order) and np.array_equal(far_ones[2], order)
+    for a, b in zip(near, far_ones):  # other alignments sum in another order: each within the bound above
+        assert np.allclose(a, b, rtol=0, atol=2.0 ** -15)
