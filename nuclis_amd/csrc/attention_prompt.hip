@@ -14,7 +14,7 @@
 // instructions to decode, as many as the softmax of 64 rows; shared by four waves
 // it is a quarter. RT is what two workgroups a CU leave room for in registers (O,
 // Q and a step's scores), since one's products then run under the other's softmax.
-// Operands are read from LDS two products ahead of their use.
+// Operands are read from LDS ahead of their use.
 //
 // Measured (4096 tokens, 48 query heads of 128 over 8, F16, 4 bits): 238 us, 866
 // TFLOP/s where a large f16 product reaches 1145 on the same card. The products alone
@@ -155,7 +155,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_prompt_kernel(CacheVi
     using G = CacheGeometry<BITS, D>;
     using S = Step<BITS, D>;
     using T = std::conditional_t<F32, float, _Float16>;
-    constexpr int PARTS = F32 ? 2 : 1, AHEAD = 2;
+    constexpr int PARTS = F32 ? 2 : 1;
+    // LDS operands on their way; one where O and Q leave no registers for two (8 bits: 251 us for a
+    // prompt of 4096 with 16 heads of 256, 460 with two of them spilling; 4 bits: 227 and 228)
+    constexpr int AHEAD = D == 256 && !F32 ? 1 : 2;
     __shared__ uint4 kb[2][S::K_OPERANDS][64], vb[2][S::V_OPERANDS][64];
     __shared__ int valid[2][4];  // of a buffer's tiles
 

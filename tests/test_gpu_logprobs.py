@@ -202,3 +202,17 @@ def test_rows_past_32_bits_of_bytes(backend):
     assert np.array_equal(near[2], order) and np.array_equal(far_ones[2], order)
     for a, b in zip(near, far_ones):  # other alignments sum in another order: each within the bound above
         assert np.allclose(a, b, rtol=0, atol=2.0 ** -15)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("top", [1, 5, 32])
+def test_rows_in_order(backend, dtype, top):
+    """Ascending rows, where every step beats all before it, and descending ones; a plateau at the bound."""
+    x = np.sort(4 * np.random.default_rng(61).standard_normal((4, 70001)), axis=1).astype(np.float32)
+    x[1] = x[1, ::-1]
+    x[2] = np.minimum(x[2], 2.0)
+    x[3] = np.round(x[3])
+    if dtype == "f16":
+        x = x.astype(np.float16).astype(np.float32)
+    targets = np.array([0, 70000, 123, 69999])
+    check(run(backend, x, targets, top, dtype), oracle(x, targets, top))
