@@ -876,19 +876,28 @@ int nuq_cache_attention(nuq_context *ctx, const nuq_cache *cache, const nuq_atte
     a.scale = n.scale * 1.44269504088896340736f;
     const uint64_t longest = n.max_length ? std::min<uint64_t>(n.max_length, a.capacity) : a.capacity;
     const uint32_t f32 = n.dtype == NUQ_F32;
+    nuq::AttentionArgs few{};
+    bool both = false;
     const auto plan_with = [&](uint64_t floats) {
-        nuq::plan_attention(cache->head_dim, cache->kv_heads, f32, longest, n.q_heads, floats, &a);
+        both = nuq::plan_attention(cache->head_dim, cache->kv_heads, f32, longest, n.q_heads, floats, &a, &few);
     };
     plan_with(UINT64_MAX);
     // without the workspace it wants (a capture, no memory): fewer splits
-    if (!ensure_workspace(ctx, a.floats)) plan_with((uint64_t)ctx->split.tiles * 256 * 256);
-    // (splits are taken where there are few workgroups: the second kernel's are fewer still)
-    if ((uint64_t)cache->kv_heads * a.splits * a.blocks * a.batch > 0x00ffffffull ||
-        (a.splits > 1 && (uint64_t)a.batch * a.max_tokens * n.q_heads > 0x00ffffffull))
+    if (!ensure_workspace(ctx, a.floats + (both ? few.floats : 0))) plan_with((uint64_t)ctx->split.tiles * 256 * 256);
+    const auto too_many = [&](const nuq::AttentionArgs &p) {
+        return (uint64_t)cache->kv_heads * p.splits * p.units > 0x00ffffffull ||
+               (p.splits > 1 && (uint64_t)p.batch * p.upto * n.q_heads > 0x00ffffffull);
+    };
+    if (too_many(a) || (both && too_many(few)))
         return fail(ctx, NUQ_INVALID_SHAPE, "too many query rows for one call");
+    e = hip_check(ctx,
+                  nuq::launch_attention(ctx->stream, view, cache->bits, cache->head_dim, f32, n.q_heads, a,
+                                        ctx->split.work),
+                  "attention launch");
+    if (e || !both) return e;
     return hip_check(ctx,
-                     nuq::launch_attention(ctx->stream, view, cache->bits, cache->head_dim, f32, n.q_heads, a,
-                                           ctx->split.work),
+                     nuq::launch_attention(ctx->stream, view, cache->bits, cache->head_dim, f32, n.q_heads, few,
+                                           ctx->split.work + a.floats),
                      "attention launch");
 }
 

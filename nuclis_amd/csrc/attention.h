@@ -22,7 +22,9 @@ struct AttentionArgs {
     float scale;          // of the scores, log2(e) among it
     // the plan
     uint32_t prompt;      // the prompt kernel's call
-    uint32_t row_tiles, blocks, splits;
+    uint32_t above, upto; // only of sequences of more than `above` and up to `upto` new tokens
+    uint32_t row_tiles, blocks, splits;  // blocks: of the rows of a sequence
+    uint64_t units;       // blocks of all sequences
     uint64_t floats;      // of workspace
     float *partial_o, *partial_ml;
 };
@@ -36,9 +38,10 @@ hipError_t launch_attention_prompt(hipStream_t s, const CacheView &c, uint32_t b
                                    const AttentionArgs &a);
 
 // Fills in the plan of a call: row tiles of 16, blocks of them, splits of the
-// long axis with at most `max_floats` of workspace.
-void plan_attention(uint32_t head_dim, uint32_t kv_heads, uint32_t f32, uint64_t max_length, uint32_t heads,
-                    uint64_t max_floats, AttentionArgs *a);
+// long axis with at most `max_floats` of workspace. Returns whether sequences of few new
+// tokens are a plan of their own, `few`, beside those of many in `a`.
+bool plan_attention(uint32_t head_dim, uint32_t kv_heads, uint32_t f32, uint64_t max_length, uint32_t heads,
+                    uint64_t max_floats, AttentionArgs *a, AttentionArgs *few);
 hipError_t launch_attention(hipStream_t s, const CacheView &c, uint32_t bits, uint32_t head_dim, uint32_t f32,
                             uint32_t heads, AttentionArgs a, float *work);
 

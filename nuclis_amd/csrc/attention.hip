@@ -197,7 +197,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_rows_kernel(CacheView
         const float inverse = whole == 0.0f ? 0.0f : 1.0f / whole;
         float *partial = nullptr;
         if (a.splits > 1) {
-            const uint64_t at = (out_row * (c.kv_heads * a.group) + out_head) * a.splits + split;
+            const uint64_t at =
+                (partial_row(a, b, s.start, token) * (c.kv_heads * a.group) + out_head) * a.splits + split;
             partial = a.partial_o + at * D;
             if ((threadIdx.x & 15) == 0) a.partial_ml[2 * at] = m, a.partial_ml[2 * at + 1] = whole;
         }
@@ -219,23 +220,39 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_rows_kernel(CacheView
     }
 }
 
+// The (sequence, token, head) of item `at` of a workgroup's ITEMS, and the place of its
+// partial results; false where there is none.
+template <uint32_t ITEMS>
+__device__ __forceinline__ bool item_of(const AttentionArgs &a, uint32_t heads, uint32_t at, uint32_t &head,
+                                        uint64_t &row, uint64_t &partial) {
+    uint32_t place = blockIdx.x, b, count = (a.upto * heads + ITEMS - 1) / ITEMS;
+    if (a.starts) {
+        if (!place_of(a, heads, ITEMS, place, b, count)) return false;
+    } else {
+        b = place / count, place %= count;
+    }
+    int begin, tokens;
+    rows_of(a, b, begin, tokens);
+    const uint32_t item = place * ITEMS + at, token = item / heads;
+    if ((int)token >= tokens) return false;
+    head = item % heads;
+    row = (uint64_t)begin + token, partial = partial_row(a, b, begin, (int)token) * heads + head;
+    return true;
+}
+
 // Joins the splits of one (sequence, token, head) a workgroup: the first wave
 // turns the splits' maxima into weights, then D / 4 threads take a split, 1024 / D
 // splits at a time. (A split without a token has sum 0 and zeros. One wave walking 64
 // splits in order took 29 us after 32768 tokens, one round of memory latency a split;
 // this takes 3.8.)
-template <int D, bool F32>
-__global__ void __launch_bounds__(256) attention_join_kernel(AttentionArgs a, uint32_t heads) {
+template <int D, bool F32> __global__ void __launch_bounds__(256) attention_join_kernel(AttentionArgs a, uint32_t heads) {
     using T = std::conditional_t<F32, float, _Float16>;
     constexpr int ACROSS = D / 4, SIDE = 256 / ACROSS;
     __shared__ float weight[MAX_SPLITS], total;
     __shared__ __align__(16) float part[SIDE][D];
-    const uint32_t head = blockIdx.x % heads, token = blockIdx.x / heads % a.max_tokens;
-    const uint32_t b = blockIdx.x / heads / a.max_tokens;
-    int begin, tokens;
-    rows_of(a, b, begin, tokens);
-    if ((int)token >= tokens) return;
-    const uint64_t row = (uint64_t)begin + token, at = row * heads + head;
+    uint32_t head;
+    uint64_t row, at;
+    if (!item_of<1>(a, heads, 0, head, row, at)) return;
     const float *ml = a.partial_ml + 2 * at * a.splits;
     const uint32_t tid = threadIdx.x;
     if (tid < 64) {
@@ -278,20 +295,16 @@ __global__ void __launch_bounds__(256) attention_join_kernel(AttentionArgs a, ui
 // call takes 149 us, 160 with a workgroup each; 8 splits about even; 32 splits of one
 // token 18.6, 16.3 with a workgroup each.)
 template <int D, bool F32>
-__global__ void __launch_bounds__(256) attention_join_rows_kernel(AttentionArgs a, uint32_t heads, uint32_t items) {
+__global__ void __launch_bounds__(256) attention_join_rows_kernel(AttentionArgs a, uint32_t heads) {
     using T = std::conditional_t<F32, float, _Float16>;
-    constexpr int ACROSS = D / 4, SIDE = 256 / ACROSS;
-    const uint32_t item = blockIdx.x * SIDE + threadIdx.x / ACROSS, x4 = 4 * (threadIdx.x % ACROSS);
-    if (item >= items) return;
-    const uint32_t head = item % heads, token = item / heads % a.max_tokens, b = item / heads / a.max_tokens;
-    int begin, tokens;
-    rows_of(a, b, begin, tokens);
-    if ((int)token >= tokens) return;
-    const uint64_t row = (uint64_t)begin + token, at = row * heads + head;
+    constexpr uint32_t ACROSS = D / 4, EACH = 4;  // splits on their way together
+    const uint32_t x4 = 4 * (threadIdx.x % ACROSS);
+    uint32_t head;
+    uint64_t row, at;
+    if (!item_of<256 / ACROSS>(a, heads, threadIdx.x / ACROSS, head, row, at)) return;
     const float *ml = a.partial_ml + 2 * at * a.splits, *p = a.partial_o + at * a.splits * D + x4;
     float4 x = make_float4(0, 0, 0, 0);
     float top = LOWEST, sum = 0.0f;
-    constexpr uint32_t EACH = 4;  // splits on their way together
     for (uint32_t first = 0; first < a.splits; first += EACH) {
         float4 y[EACH];
         float m[EACH], l[EACH];
@@ -319,7 +332,7 @@ __global__ void __launch_bounds__(256) attention_join_rows_kernel(AttentionArgs 
 
 template <int BITS, int D, int RT, bool F32>
 hipError_t rows_launch(hipStream_t s, const CacheView &c, const AttentionArgs &a) {
-    const uint32_t grid = c.kv_heads * a.splits * a.blocks * a.batch;
+    const uint32_t grid = (uint32_t)(c.kv_heads * a.splits * a.units);
     attention_rows_kernel<BITS, D, RT, F32><<<grid, 64 * WAVES, 0, s>>>(c, a);
     return hipGetLastError();
 }
@@ -353,57 +366,103 @@ template <bool F32> hipError_t rows_dispatch(hipStream_t s, const CacheView &c, 
 // way through memory. Rows: up to 512 tokens are one workgroup's (300 tokens: 6.6
 // us, 7.7 split in three and joined); then 128 tokens each while a workgroup a CU wants
 // work (4096 tokens: 8.1 us, 10.5 at 512 each), and four a CU where each has 1024
-// (batch of 32 up to 16384: 83 us, 88 at two a CU, 114 at one). Prompts: three
-// workgroups a CU of 1024 tokens and more, where rows are few against the tokens they
-// see (512 tokens after 8192, F32: 221 us, 267 at two a CU; F16: 143, 285 unsplit; a prompt
-// of 2000 164 split, 86 not) or heads are wide (3000 tokens at D = 256: 160 and 193).
-void plan_attention(uint32_t head_dim, uint32_t kv_heads, uint32_t f32, uint64_t max_length, uint32_t heads,
-                    uint64_t max_floats, AttentionArgs *a) {
+// (batch of 32 up to 16384: 83 us, 88 at two a CU, 114 at one). Prompts: where
+// rows are few against the tokens they see, n that makes the least of (rounds of the 512
+// workgroups that run at once) / n and what joining n costs, 170 n / tokens (300 tokens
+// after 16000, F16, 80 workgroups: 196 us in 3, 156 in 6, 196 in 7; 1000, 256 workgroups: 411 in
+// 2, 424 in 4; a window of 4096 at D = 256, 256 workgroups: 206 in 2, 239 in 4). A prompt from its
+// start on is in balance by itself (2000 tokens: 164 us split, 86 not), but for wide
+// heads (4096 tokens at D = 256, 512 workgroups: 294 us, 222 in 2).
+//
+// A batch of both, single tokens among prompts, is two plans where its other sequences
+// are short (at most 256 rows each beside the longest): up to 64 rows by rows, the
+// others by the prompt kernel (a prompt of 512 among 32 single tokens after 8000: 120 us, all
+// by the prompt kernel 738; calls of their own, which know each other's lengths, 78).
+// Units of a call whose sequences bring up to `most` tokens, ceil(tokens * by / of) each.
+static uint64_t units_of(const AttentionArgs &a, uint64_t by, uint64_t of) {
+    const uint64_t all = a.batch * ((a.upto * by + of - 1) / of);
+    // sequences have more than `above` tokens, and none of them more than a unit that is not full
+    const uint64_t sequences = std::min<uint64_t>(a.batch, a.rows / (a.above + 1));
+    return a.starts ? std::min(all, a.rows * by / of + sequences) : all;
+}
+static uint64_t rows_splits(uint64_t groups, uint64_t reach) {
+    if (reach <= 512) return 1;
+    return std::max(std::min(256 / groups, (reach + 127) / 128), std::min(1024 / groups, (reach + 1023) / 1024));
+}
+static void fit_splits(uint64_t splits, uint64_t rows, uint32_t heads, uint32_t head_dim, uint64_t max_floats,
+                       AttentionArgs *a) {
+    splits = std::max<uint64_t>(1, std::min<uint64_t>(splits, MAX_SPLITS));
+    const uint64_t each = rows * heads * (head_dim + 2);
+    if (splits > 1 && splits * each > max_floats) splits = std::max<uint64_t>(1, max_floats / each);
+    a->splits = (uint32_t)splits;
+    a->floats = splits > 1 ? (splits * each + 3) / 4 * 4 : 0;  // another plan's may follow, 16-byte aligned
+}
+bool plan_attention(uint32_t head_dim, uint32_t kv_heads, uint32_t f32, uint64_t max_length, uint32_t heads,
+                    uint64_t max_floats, AttentionArgs *a, AttentionArgs *few) {
     const uint64_t rows = (uint64_t)a->max_tokens * a->group;
     uint64_t reach = max_length;  // tokens the last row and those before it may see
     if (a->window) reach = std::min<uint64_t>(reach, (uint64_t)a->window + a->max_tokens);
     const double seen = std::max((double)reach - 0.5 * a->max_tokens, 0.5 * (double)reach);
-    const double work = (double)a->batch * a->max_tokens * heads * seen * head_dim;
+    const double work = (double)a->rows * heads * seen * head_dim;
+    a->above = 0, a->upto = a->max_tokens;
     a->prompt = rows > 64 && work >= (f32 || head_dim == 64 ? 1.2e10 : 8e9);
-    if (a->prompt) {
-        a->row_tiles = prompt_row_tiles((int)head_dim, f32) * WAVES;
-    } else {
-        a->row_tiles = head_dim <= 128 && rows > 16 ? 2 : 1;
-    }
+    const auto tiles_of = [&](uint64_t n) { return head_dim <= 128 && n > 16 ? 2u : 1u; };
+    a->row_tiles = a->prompt ? prompt_row_tiles((int)head_dim, f32) * WAVES : tiles_of(rows);
     a->blocks = (uint32_t)((rows + 16 * a->row_tiles - 1) / (16 * a->row_tiles));
-    const uint64_t groups = (uint64_t)a->batch * kv_heads * a->blocks;
-    uint64_t splits = 1;
-    if (a->prompt) {
-        if (reach >= 4ull * a->max_tokens || head_dim == 256) splits = std::min((768 + groups - 1) / groups, reach / 1024);
-    } else if (reach > 512) {
-        splits = std::max(std::min(256 / groups, (reach + 127) / 128), std::min(1024 / groups, (reach + 1023) / 1024));
+    a->units = (uint64_t)a->batch * a->blocks;
+    if (!a->prompt) {
+        fit_splits(rows_splits((uint64_t)kv_heads * a->units, reach), a->rows, heads, head_dim, max_floats, a);
+        return false;
     }
-    splits = std::max<uint64_t>(1, std::min<uint64_t>(splits, MAX_SPLITS));
-    const uint64_t each = (uint64_t)a->rows * heads * (head_dim + 2);
-    if (splits > 1 && splits * each > max_floats) splits = std::max<uint64_t>(1, max_floats / each);
-    a->splits = (uint32_t)splits;
-    a->floats = splits > 1 ? splits * each : 0;
+    const uint64_t others = a->rows > a->max_tokens ? a->rows - a->max_tokens : 0;  // tokens beside the longest's
+    const uint32_t few_tokens = 64 / a->group;
+    const bool both = a->starts && a->batch > 1 && few_tokens && others * a->group <= 256ull * (a->batch - 1);
+    if (both) {
+        *few = *a;
+        few->prompt = 0, few->upto = few_tokens, a->above = few_tokens;
+        few->row_tiles = 1;  // most bring one token
+        few->blocks = (few_tokens * a->group + 15) / 16;
+        few->units = (uint64_t)few->batch * few->blocks;
+        fit_splits(rows_splits((uint64_t)a->batch * kv_heads, reach), (uint64_t)a->batch * few_tokens, heads, head_dim,
+                   max_floats, few);
+        max_floats -= few->floats;
+    }
+    a->units = units_of(*a, a->group, 16 * a->row_tiles);
+    // the longest's units, and the others' taken for half as long (none where they are the other plan's)
+    const uint64_t others_units = both ? 0 : a->units - std::min<uint64_t>(a->units, a->blocks);
+    const uint64_t busy = kv_heads * (std::min<uint64_t>(a->units, a->blocks) + (a->starts ? (others_units + 1) / 2 : others_units));
+    uint64_t splits = 1;
+    if (reach >= 4ull * a->max_tokens) {
+        double least = 1e30;
+        for (uint64_t n = 1; n <= std::max<uint64_t>(1, std::min<uint64_t>(reach / 1024, MAX_SPLITS)); ++n) {
+            const double cost = (double)((busy * n + 511) / 512) / n + 170.0 * n / reach;
+            if (cost < least) least = cost, splits = n;
+        }
+    } else if (head_dim == 256) {
+        splits = std::min((640 + busy - 1) / busy, reach / 1024);
+    }
+    fit_splits(splits, a->rows, heads, head_dim, max_floats, a);
+    return both;
 }
 
 hipError_t launch_attention(hipStream_t s, const CacheView &c, uint32_t bits, uint32_t head_dim, uint32_t f32,
                             uint32_t heads, AttentionArgs a, float *work) {
     if (a.splits > 1) {
         a.partial_o = work;
-        a.partial_ml = work + (uint64_t)a.rows * heads * a.splits * head_dim;
+        a.partial_ml = work + a.floats / (head_dim + 2) * head_dim;
     }
     const hipError_t e = a.prompt ? launch_attention_prompt(s, c, bits, head_dim, f32, a)
                          : f32    ? rows_dispatch<true>(s, c, bits, head_dim, a)
                                   : rows_dispatch<false>(s, c, bits, head_dim, a);
     if (e != hipSuccess || a.splits == 1) return e;
-    const uint32_t items = a.batch * a.max_tokens * heads;
     const bool few_splits = a.splits <= 8;
-#define NUQ_CASE(D)                                                                                              \
-    if (head_dim == D) {                                                                                         \
-        const uint32_t grid = (items + 1024 / D - 1) / (1024 / D);                                                \
-        if (few_splits && f32) attention_join_rows_kernel<D, true><<<grid, 256, 0, s>>>(a, heads, items);                \
-        else if (few_splits) attention_join_rows_kernel<D, false><<<grid, 256, 0, s>>>(a, heads, items);                 \
-        else if (f32) attention_join_kernel<D, true><<<items, 256, 0, s>>>(a, heads);                            \
-        else attention_join_kernel<D, false><<<items, 256, 0, s>>>(a, heads);                                    \
+    const uint32_t grid = (uint32_t)units_of(a, heads, few_splits ? 1024 / head_dim : 1);
+#define NUQ_CASE(D)                                                                             \
+    if (head_dim == D) {                                                                        \
+        if (few_splits && f32) attention_join_rows_kernel<D, true><<<grid, 256, 0, s>>>(a, heads); \
+        else if (few_splits) attention_join_rows_kernel<D, false><<<grid, 256, 0, s>>>(a, heads);  \
+        else if (f32) attention_join_kernel<D, true><<<grid, 256, 0, s>>>(a, heads);            \
+        else attention_join_kernel<D, false><<<grid, 256, 0, s>>>(a, heads);                    \
     }
     NUQ_CASE(64) NUQ_CASE(128) NUQ_CASE(256)
 #undef NUQ_CASE

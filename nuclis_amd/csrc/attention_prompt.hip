@@ -169,7 +169,12 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_prompt_kernel(CacheVi
     id /= c.kv_heads;
     const uint32_t split = id % a.splits;
     id /= a.splits;
-    const uint32_t block = a.blocks - 1 - id % a.blocks, b = id / a.blocks;
+    uint32_t b = id / a.blocks, place = id % a.blocks, blocks = a.blocks;
+    if (a.starts) {
+        place = id;
+        if (!place_of(a, a.group, 16 * RT * WAVES, place, b, blocks)) return;
+    }
+    const uint32_t block = blocks - 1 - place;
     Span s;
     if (!span_of<16 * RT * WAVES, S::TOKENS>(a, b, block, split, s)) return;
     const PageTable table = table_of(a, b);
@@ -268,7 +273,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_prompt_kernel(CacheVi
         const uint64_t out_row = (uint64_t)(s.start + token);
         const uint32_t out_head = head * a.group + row - token * a.group;
         const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
-        const uint64_t at = (out_row * (c.kv_heads * a.group) + out_head) * a.splits + split;
+        const uint64_t at =
+            (partial_row(a, b, s.start, token) * (c.kv_heads * a.group) + out_head) * a.splits + split;
         if (a.splits > 1 && h == 0) a.partial_ml[2 * at] = rows.top[t], a.partial_ml[2 * at + 1] = l;
 #pragma unroll
         for (int u = 0; u < G::UNITS; ++u)
@@ -287,7 +293,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_prompt_kernel(CacheVi
 
 template <int BITS, int D, bool F32> hipError_t prompt_launch(hipStream_t s, const CacheView &c, const AttentionArgs &a) {
     constexpr int RT = prompt_row_tiles(D, F32);
-    const uint32_t grid = c.kv_heads * a.splits * a.blocks * a.batch;
+    const uint32_t grid = (uint32_t)(c.kv_heads * a.splits * a.units);
     attention_prompt_kernel<BITS, D, RT, F32><<<grid, 64 * WAVES, 0, s>>>(c, a);
     return hipGetLastError();
 }

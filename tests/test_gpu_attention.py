@@ -308,7 +308,7 @@ def prompt_table(c):
     cache once for four waves takes it, split over workgroups, however short it is."""
     brought, heads = max(c.brought), c.kv * c.group
     assert brought * c.group > 64
-    wide = -(-int(1.3e10 / (len(c.held) * brought * heads * c.d)) // c.page) + 1
+    wide = -(-int(1.3e10 / (sum(c.brought) * heads * c.d)) // c.page) + 1
     table = np.full((len(c.held), max(wide, c.table.shape[1])), -1, np.int32)
     table[:, :c.table.shape[1]] = c.table
     return table
@@ -456,3 +456,20 @@ def test_offsets_past_32_bits(backend, tokens):
     q.copy_(to_gpu(c.q))
     out.fill_(7.0)
     assert np.array_equal(c.run(backend, table=moved, q=q, out=out), want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("d,kv,group", [(64, 1, 6), (128, 2, 3), (256, 1, 12)])
+def test_prompts_among_single_tokens_and_drafts(backend, dtype, d, kv, group):
+    """More sequences than a wave has lanes, some of many tokens, some of one, a few or none, each
+    kind with its own splits and partial results."""
+    rng = np.random.default_rng(24)
+    brought = [1] * 85
+    brought[3], brought[40], brought[66], brought[84] = 130, 64 // group + 1, 77, 64 // group
+    brought[10] = brought[64] = 0
+    held = [int(n) for n in rng.integers(1, 400, 85)]
+    held[3], held[5], held[66], held[70], held[84] = 700, 0, 77, 1500, 900
+    c = Case(held, brought, d=d, kv=kv, group=group, page=16, dtype=dtype, seed=25)
+    got = c.run(backend, table=prompt_table(c))
+    c.check(got)
+    c.check(c.run(backend, window=150), window=150)
