@@ -190,7 +190,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_rows_kernel(CacheView
         for (int w = 1; w < WAVES; ++w) m = fmaxf(m, merge_m[w][r]);
         float by[WAVES], whole = 0.0f;
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) by[w] = __builtin_amdgcn_exp2f(merge_m[w][r] - m), whole += by[w] * merge_l[w][r];
+        for (int w = 0; w < WAVES; ++w) {
+            by[w] = __builtin_amdgcn_exp2f(merge_m[w][r] - m);
+            whole += by[w] * merge_l[w][r];
+        }
         const int token = row / (int)a.group;
         const uint64_t out_row = (uint64_t)(s.start + token);
         const uint32_t out_head = head * a.group + row - token * a.group;
@@ -245,7 +248,8 @@ __device__ __forceinline__ bool item_of(const AttentionArgs &a, uint32_t heads, 
 // splits at a time. (A split without a token has sum 0 and zeros. One wave walking 64
 // splits in order took 29 us after 32768 tokens, one round of memory latency a split;
 // this takes 3.8.)
-template <int D, bool F32> __global__ void __launch_bounds__(256) attention_join_kernel(AttentionArgs a, uint32_t heads) {
+template <int D, bool F32>
+__global__ void __launch_bounds__(256) attention_join_kernel(AttentionArgs a, uint32_t heads) {
     using T = std::conditional_t<F32, float, _Float16>;
     constexpr int ACROSS = D / 4, SIDE = 256 / ACROSS;
     __shared__ float weight[MAX_SPLITS], total;
@@ -355,6 +359,29 @@ template <bool F32> hipError_t rows_dispatch(hipStream_t s, const CacheView &c, 
 
 }  // namespace
 
+// At least the units of all of a plan's sequences, ceil(tokens * by / of) each.
+static uint64_t units_of(const AttentionArgs &a, uint64_t by, uint64_t of) {
+    const uint64_t all = a.batch * ((a.upto * by + of - 1) / of);
+    // sequences have more than `above` tokens, and none of them more than a unit that is not full
+    const uint64_t sequences = std::min<uint64_t>(a.batch, a.rows / (a.above + 1));
+    return a.starts ? std::min(all, a.rows * by / of + sequences) : all;
+}
+// The splits of the rows kernel's calls (plan_attention).
+static uint64_t rows_splits(uint64_t groups, uint64_t reach) {
+    if (reach <= 512) return 1;
+    return std::max(std::min(256 / groups, (reach + 127) / 128), std::min(1024 / groups, (reach + 1023) / 1024));
+}
+// Sets the splits, as far as their partial results of `rows` query rows fit.
+static void fit_splits(uint64_t splits, uint64_t rows, uint32_t heads, uint32_t head_dim, uint64_t max_floats,
+                       AttentionArgs *a) {
+    splits = std::max<uint64_t>(1, std::min<uint64_t>(splits, MAX_SPLITS));
+    const uint64_t each = rows * heads * (head_dim + 2);
+    max_floats = std::min<uint64_t>(max_floats, 1ull << 26);  // 256 MiB of partial results
+    if (splits > 1 && splits * each > max_floats) splits = std::max<uint64_t>(1, max_floats / each);
+    a->splits = (uint32_t)splits;
+    a->floats = splits > 1 ? (splits * each + 3) / 4 * 4 : 0;  // another plan's may follow, 16-byte aligned
+}
+
 // The kernel. Few rows read the cache straight into registers; where there is enough
 // work for it, a workgroup that decodes the cache once for its waves is faster:
 // 48 heads of 128, F16: one prompt of 1000 tokens 39 us by rows, 46 by the prompt
@@ -378,25 +405,6 @@ template <bool F32> hipError_t rows_dispatch(hipStream_t s, const CacheView &c, 
 // are short (at most 256 rows each beside the longest): up to 64 rows by rows, the
 // others by the prompt kernel (a prompt of 512 among 32 single tokens after 8000: 120 us, all
 // by the prompt kernel 738; calls of their own, which know each other's lengths, 78).
-// Units of a call whose sequences bring up to `most` tokens, ceil(tokens * by / of) each.
-static uint64_t units_of(const AttentionArgs &a, uint64_t by, uint64_t of) {
-    const uint64_t all = a.batch * ((a.upto * by + of - 1) / of);
-    // sequences have more than `above` tokens, and none of them more than a unit that is not full
-    const uint64_t sequences = std::min<uint64_t>(a.batch, a.rows / (a.above + 1));
-    return a.starts ? std::min(all, a.rows * by / of + sequences) : all;
-}
-static uint64_t rows_splits(uint64_t groups, uint64_t reach) {
-    if (reach <= 512) return 1;
-    return std::max(std::min(256 / groups, (reach + 127) / 128), std::min(1024 / groups, (reach + 1023) / 1024));
-}
-static void fit_splits(uint64_t splits, uint64_t rows, uint32_t heads, uint32_t head_dim, uint64_t max_floats,
-                       AttentionArgs *a) {
-    splits = std::max<uint64_t>(1, std::min<uint64_t>(splits, MAX_SPLITS));
-    const uint64_t each = rows * heads * (head_dim + 2);
-    if (splits > 1 && splits * each > max_floats) splits = std::max<uint64_t>(1, max_floats / each);
-    a->splits = (uint32_t)splits;
-    a->floats = splits > 1 ? (splits * each + 3) / 4 * 4 : 0;  // another plan's may follow, 16-byte aligned
-}
 bool plan_attention(uint32_t head_dim, uint32_t kv_heads, uint32_t f32, uint64_t max_length, uint32_t heads,
                     uint64_t max_floats, AttentionArgs *a, AttentionArgs *few) {
     const uint64_t rows = (uint64_t)a->max_tokens * a->group;
@@ -430,7 +438,8 @@ bool plan_attention(uint32_t head_dim, uint32_t kv_heads, uint32_t f32, uint64_t
     a->units = units_of(*a, a->group, 16 * a->row_tiles);
     // the longest's units, and the others' taken for half as long (none where they are the other plan's)
     const uint64_t others_units = both ? 0 : a->units - std::min<uint64_t>(a->units, a->blocks);
-    const uint64_t busy = kv_heads * (std::min<uint64_t>(a->units, a->blocks) + (a->starts ? (others_units + 1) / 2 : others_units));
+    const uint64_t busy = kv_heads * (std::min<uint64_t>(a->units, a->blocks) +
+                                      (a->starts ? (others_units + 1) / 2 : others_units));
     uint64_t splits = 1;
     if (reach >= 4ull * a->max_tokens) {
         double least = 1e30;

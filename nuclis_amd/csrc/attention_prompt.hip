@@ -157,8 +157,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_prompt_kernel(CacheVi
     using T = std::conditional_t<F32, float, _Float16>;
     constexpr int PARTS = F32 ? 2 : 1;
     // LDS operands on their way; one where O and Q leave no registers for two (8 bits: 251 us for a
-    // prompt of 4096 with 16 heads of 256, 460 with two of them spilling; 4 bits: 227 and 228)
-    constexpr int AHEAD = D == 256 && !F32 ? 1 : 2;
+    // prompt of 4096 with 16 heads of 256, 460 with two of them spilling; at 4 bits two
+    // are as fast, 149 and 151 us for two chunks of 1000 over a window)
+    constexpr int AHEAD = D == 256 && BITS == 8 && !F32 ? 1 : 2;
     __shared__ uint4 kb[2][S::K_OPERANDS][64], vb[2][S::V_OPERANDS][64];
     __shared__ int valid[2][4];  // of a buffer's tiles
 
@@ -227,7 +228,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_prompt_kernel(CacheVi
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int t = 0; t < RT; ++t) x[i][t] = floatx4{0, 0, 0, 0};
-                const uint4(*const k)[64] = kb[buffer] + 2 * pair * G::GROUPS, (*const v)[64] = vb[buffer] + pair * (D / 16);
+                const uint4(*const k)[64] = kb[buffer] + 2 * pair * G::GROUPS;
+                const uint4(*const v)[64] = vb[buffer] + pair * (D / 16);
                 __builtin_amdgcn_sched_barrier(0);
                 uint4 ahead[AHEAD];
 #pragma unroll
@@ -243,7 +245,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_prompt_kernel(CacheVi
                 }
                 if (masked) {
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) rows.mask(x[i], first + 32 * pair + 16 * i + 4 * h, there[2 * pair + i]);
+                    for (int i = 0; i < 2; ++i)
+                        rows.mask(x[i], first + 32 * pair + 16 * i + 4 * h, there[2 * pair + i]);
                 }
                 Operand p[PARTS][RT];
                 rows.template raise<2>(x);

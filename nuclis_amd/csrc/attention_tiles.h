@@ -432,7 +432,8 @@ template <int BITS, int D, int RT, bool F32> struct Rows {
         if (__any(past)) {
 #pragma unroll
             for (int t = 0; t < RT; ++t) {
-                const float higher = fmaxf(top[t], over_quarters_max(most[t])), by = __builtin_amdgcn_exp2f(top[t] - higher);
+                const float higher = fmaxf(top[t], over_quarters_max(most[t]));
+                const float by = __builtin_amdgcn_exp2f(top[t] - higher);
                 top[t] = higher;
                 sum[t] *= by;
 #pragma unroll

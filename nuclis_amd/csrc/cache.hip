@@ -185,14 +185,16 @@ __global__ void __launch_bounds__(256) cache_write_kernel(CacheView c, const T *
 }
 
 // The 4 codes, as they stand with their offset, of dimensions 4 * quad ..+3 of token n.
-template <int BITS, int D> __device__ __forceinline__ void k_quad(const uint8_t *tile, int n, int quad, uint32_t (&q)[4]) {
+template <int BITS, int D>
+__device__ __forceinline__ void k_quad(const uint8_t *tile, int n, int quad, uint32_t (&q)[4]) {
     const uint8_t *p = tile + Place<BITS, D>::k_codes(n, quad >> 1);
     const uint32_t w = *(const uint32_t *)(BITS == 4 ? p : p + 4 * (quad & 1)), by = BITS == 4 ? 8 * (quad & 1) : 0;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         q[e] = BITS == 4 ? w >> (by + 4 * (e >> 1) + 16 * (e & 1)) & 15u : w >> (8 * e) & 255u;
 }
-template <int BITS, int D> __device__ __forceinline__ void v_quad(const uint8_t *tile, int n, int quad, uint32_t (&q)[4]) {
+template <int BITS, int D>
+__device__ __forceinline__ void v_quad(const uint8_t *tile, int n, int quad, uint32_t (&q)[4]) {
     using P = Place<BITS, D>;
     const uint8_t *p = tile + P::v_codes(n, quad >> 1);
     uint32_t w;
@@ -212,7 +214,8 @@ __global__ void __launch_bounds__(256) cache_read_kernel(CacheView c, const int6
     using G = CacheGeometry<BITS, D>;
     using P = Place<BITS, D>;
     typedef T vector __attribute__((ext_vector_type(16 / sizeof(T))));
-    constexpr int LANES = D / 8, QUADS = sizeof(T) == 2 ? 2 : 1, PASSES = sizeof(T) / 2;  // D / 8 lanes: twice 4 or once 8
+    // D / 8 lanes hold a token-head: F32 in two passes of 4 dimensions, F16 in one of 8
+    constexpr int LANES = D / 8, QUADS = sizeof(T) == 2 ? 2 : 1, PASSES = sizeof(T) / 2;
     const uint32_t head = blockIdx.x % c.kv_heads;
     const uint64_t t = (uint64_t)(blockIdx.x / c.kv_heads) * (256 / LANES) + threadIdx.x / LANES;
     if (t >= tokens) return;
