@@ -234,8 +234,8 @@ __device__ __forceinline__ bool item_of(const AttentionArgs &a, uint32_t heads, 
     } else {
         b = place / count, place %= count;
     }
-    int begin, tokens;
-    rows_of(a, b, begin, tokens);
+    int begin, tokens, brought;
+    rows_of(a, b, begin, tokens, brought);
     const uint32_t item = place * ITEMS + at, token = item / heads;
     if ((int)token >= tokens) return false;
     head = item % heads;

@@ -213,13 +213,16 @@ struct Span {
     int low, high;    // steps of this split
 };
 
-// The query rows of sequence b, whatever `starts` holds.
-__device__ __forceinline__ void rows_of(const AttentionArgs &a, uint32_t b, int &begin, int &tokens) {
+// The query rows of sequence b, whatever `starts` holds. `brought` are its new tokens, of
+// which the first `tokens` have rows that are computed: they stand before the others.
+__device__ __forceinline__ void rows_of(const AttentionArgs &a, uint32_t b, int &begin, int &tokens, int &brought) {
     begin = (int)(b * a.max_tokens);
-    tokens = (int)a.max_tokens;
+    tokens = brought = (int)a.max_tokens;
     if (a.starts) {
         begin = min(max(a.starts[b], 0), (int)a.rows);
-        tokens = min(min(max(a.starts[b + 1], begin), (int)a.rows) - begin, (int)a.max_tokens);
+        const int end = max(a.starts[b + 1], begin);
+        brought = end - begin;
+        tokens = min(min(end, (int)a.rows) - begin, (int)a.max_tokens);
         if (tokens <= (int)a.above || tokens > (int)a.upto) tokens = 0;
     }
 }
@@ -239,8 +242,8 @@ __device__ __forceinline__ bool place_of(const AttentionArgs &a, uint32_t by, ui
                                          uint32_t &count) {
     const int lane = (int)threadIdx.x & 63;
     for (uint32_t first = 0; first < a.batch; first += 64) {
-        int begin, tokens = 0;
-        if (first + lane < a.batch) rows_of(a, first + lane, begin, tokens);
+        int begin, tokens = 0, brought;
+        if (first + lane < a.batch) rows_of(a, first + lane, begin, tokens, brought);
         const uint32_t own = ((uint32_t)tokens * by + of - 1) / of;
         uint32_t sum = own;  // of this lane's and all before it
 #pragma unroll
@@ -264,19 +267,21 @@ __device__ __forceinline__ bool place_of(const AttentionArgs &a, uint32_t by, ui
 // The rows and steps of a workgroup; false where it has no rows.
 template <int ROWS, int STEP>
 __device__ __forceinline__ bool span_of(const AttentionArgs &a, uint32_t b, uint32_t block, uint32_t split, Span &s) {
-    int tokens;
-    rows_of(a, b, s.start, tokens);
+    int tokens, brought;
+    rows_of(a, b, s.start, tokens, brought);
     s.rows = tokens * (int)a.group;
     s.first_row = (int)block * ROWS;
     if (s.first_row >= s.rows) return false;
     const int length = min(max(a.lengths[b], 0), (int)a.capacity);
-    s.position = length - tokens;
+    // (a start before -tokens leaves the rows nothing, as -tokens does)
+    s.position = length - min(brought, length + tokens);
     const int token_low = s.first_row / (int)a.group;
     const int token_high = min(s.first_row + ROWS - 1, s.rows - 1) / (int)a.group;
     s.to = max(s.position + token_high + 1, 0);
     // the window may be as large as an int holds: no sum may pass it
     s.from = a.window ? max(s.position + token_low - (int)a.window + 1, 0) : 0;
-    const int begin_step = s.from / STEP, steps = s.to > s.from ? (s.to + STEP - 1) / STEP - begin_step : 0;
+    const int begin_step = s.to > s.from ? s.from / STEP : 0;
+    const int steps = s.to > s.from ? (s.to + STEP - 1) / STEP - begin_step : 0;
     const int each = (steps + (int)a.splits - 1) / (int)a.splits;
     s.low = begin_step + min((int)split * each, steps);
     s.high = begin_step + min(((int)split + 1) * each, steps);

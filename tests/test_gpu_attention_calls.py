@@ -1,0 +1,54 @@
+"""Calls of the attention over the quantised cache whose bounds are not the batch's own
+counts (nuq_cache_attention, include/nuq.h), against the float64 oracle under the
+bounds of test_gpu_attention.py."""
+import numpy as np
+import pytest
+
+import nuclis_amd as nq
+from tests.gpu_util import to_gpu
+from tests.test_gpu_attention import Case, prompt_table
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def backend():
+    import torch
+    assert torch.cuda.is_available(), "GPU tests need a GPU"
+    return nq.Backend(0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("window", [0, 21])
+def test_rows_before_a_bound_keep_their_positions(backend, dtype, window):
+    """Sequences of more new tokens than max_tokens: the rows before it see what they see without
+    the bound, the others stay as they are."""
+    c = Case([40, 50, 3], [4, 4, 4], kv=1, group=2, d=64, page=16, dtype=dtype, seed=8)
+    c.check(c.run(backend, window=window), window=window)
+    got = c.run(backend, starts=np.array([0, 4, 8, 12]), max_tokens=2, window=window)
+    c.check(got, window=window, rows=np.arange(2))
+    for b in range(3):
+        assert np.all(got[4 * b + 2:4 * b + 4] == 7.0)
+    assert not got[8:9].any()  # the third one's first token stands before its start
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("window", [0, 45])
+def test_prompt_rows_before_a_bound_keep_their_positions(backend, dtype, window):
+    c = Case([531, 90], [70, 80], kv=1, group=3, page=16, dtype=dtype, seed=26)
+    got = c.run(backend, starts=np.array([0, 70, 150]), max_tokens=66, table=prompt_table(c), window=window)
+    c.check(got, window=window, rows=np.arange(66))
+    assert np.all(got[66:70] == 7.0) and np.all(got[136:] == 7.0)
+
+
+@pytest.mark.parametrize("prompt", [False, True])
+def test_rows_before_the_end_of_the_queries_keep_their_positions(backend, prompt):
+    """Starts that name more rows than there are."""
+    c = Case([300, 120], [30, 40], kv=1, group=3, page=16, seed=27)
+    q = to_gpu(c.q)[:55].contiguous()
+    got = c.run(backend, q=q, starts=np.array([0, 30, 70]), max_tokens=40,
+                **(dict(table=prompt_table(c)) if prompt else {}))
+    c.check(np.concatenate([got, np.zeros((15, 3, 128))]), rows=np.arange(25))
+    # a count past any the sequence can hold: every row stands before its start
+    got = c.run(backend, q=q, starts=np.array([0, 30, 2**31 - 1]), max_tokens=40)
+    assert not got[30:].any()
