@@ -884,9 +884,8 @@ int nuq_cache_attention(nuq_context *ctx, const nuq_cache *cache, const nuq_atte
     plan_with(UINT64_MAX);
     // without the workspace it wants (a capture, no memory): fewer splits
     if (!ensure_workspace(ctx, a.floats + (both ? few.floats : 0))) plan_with((uint64_t)ctx->split.tiles * 256 * 256);
-    const auto too_many = [&](const nuq::AttentionArgs &p) {
-        return (uint64_t)cache->kv_heads * p.splits * p.units > 0x00ffffffull ||
-               (p.splits > 1 && (uint64_t)p.batch * p.upto * n.q_heads > 0x00ffffffull);
+    const auto too_many = [&](const nuq::AttentionArgs &p) {  // (splits are already cut to what a launch takes)
+        return (uint64_t)cache->kv_heads * p.splits * p.units > nuq::MOST_GROUPS;
     };
     if (too_many(a) || (both && too_many(few)))
         return fail(ctx, NUQ_INVALID_SHAPE, "too many query rows for one call");

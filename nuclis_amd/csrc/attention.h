@@ -37,6 +37,9 @@ constexpr int prompt_tokens(int head_dim) { return head_dim == 256 ? 32 : 64; }
 hipError_t launch_attention_prompt(hipStream_t s, const CacheView &c, uint32_t bits, uint32_t d, uint32_t f32,
                                    const AttentionArgs &a);
 
+// The most workgroups of a launch, 256 threads each (2^32 threads in all).
+constexpr uint64_t MOST_GROUPS = 0x00ffffffull;
+
 // Fills in the plan of a call: row tiles of 16, blocks of them, splits of the
 // long axis with at most `max_floats` of workspace. Returns whether sequences of few new
 // tokens are a plan of their own, `few`, beside those of many in `a`.

@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(AttentionArgs a, ui
     store4((T *)a.out + row * a.out_stride + head * D + x4, x, inverse);
 }
 
-// The same where splits are few (up to 8): D / 4 threads take a (sequence, token, head) and
+// The same where splits are few (FEW_SPLITS, 8): D / 4 threads take a (sequence, token, head) and
 // walk them, four on their way together. (2 x 1000 tokens of 16 heads of 256 in three splits: the
 // call takes 149 us, 160 with a workgroup each; 8 splits about even; 32 splits of one
 // token 18.6, 16.3 with a workgroup each.)
@@ -371,13 +371,22 @@ static uint64_t rows_splits(uint64_t groups, uint64_t reach) {
     if (reach <= 512) return 1;
     return std::max(std::min(256 / groups, (reach + 127) / 128), std::min(1024 / groups, (reach + 1023) / 1024));
 }
-// Sets the splits, as far as their partial results of `rows` query rows fit.
-static void fit_splits(uint64_t splits, uint64_t rows, uint32_t heads, uint32_t head_dim, uint64_t max_floats,
-                       AttentionArgs *a) {
-    splits = std::max<uint64_t>(1, std::min<uint64_t>(splits, MAX_SPLITS));
+// Workgroups of the kernel that joins a plan's splits: D / 4 threads a (row, head) where they are
+// few, a workgroup each where they are many.
+constexpr uint32_t FEW_SPLITS = 8;
+static uint64_t join_groups(const AttentionArgs &a, uint32_t heads, uint32_t head_dim, uint64_t splits) {
+    return units_of(a, heads, splits <= FEW_SPLITS ? 1024 / head_dim : 1);
+}
+// Sets the splits, as far as their partial results of `rows` query rows fit and neither kernel's
+// grid passes a launch's.
+static void fit_splits(uint64_t splits, uint64_t rows, uint32_t kv_heads, uint32_t heads, uint32_t head_dim,
+                       uint64_t max_floats, AttentionArgs *a) {
+    splits = std::min<uint64_t>(std::min<uint64_t>(splits, MAX_SPLITS), MOST_GROUPS / (kv_heads * a->units));
+    splits = std::max<uint64_t>(1, splits);
     const uint64_t each = rows * heads * (head_dim + 2);
     max_floats = std::min<uint64_t>(max_floats, 1ull << 26);  // 256 MiB of partial results
     if (splits > 1 && splits * each > max_floats) splits = std::max<uint64_t>(1, max_floats / each);
+    if (splits > 1 && join_groups(*a, heads, head_dim, splits) > MOST_GROUPS) splits = 1;
     a->splits = (uint32_t)splits;
     a->floats = splits > 1 ? (splits * each + 3) / 4 * 4 : 0;  // another plan's may follow, 16-byte aligned
 }
@@ -413,13 +422,17 @@ bool plan_attention(uint32_t head_dim, uint32_t kv_heads, uint32_t f32, uint64_t
     const double seen = std::max((double)reach - 0.5 * a->max_tokens, 0.5 * (double)reach);
     const double work = (double)a->rows * heads * seen * head_dim;
     a->above = 0, a->upto = a->max_tokens;
-    a->prompt = rows > 64 && work >= (f32 || head_dim == 64 ? 1.2e10 : 8e9);
     const auto tiles_of = [&](uint64_t n) { return head_dim <= 128 && n > 16 ? 2u : 1u; };
+    // (the rows kernel's grid has every sequence's blocks for max_tokens; the prompt kernel's, where counts
+    // differ, is sized by the rows there are)
+    const uint64_t rows_groups = kv_heads * (uint64_t)a->batch * ((rows + 16 * tiles_of(rows) - 1) / (16 * tiles_of(rows)));
+    a->prompt = rows > 64 && (work >= (f32 || head_dim == 64 ? 1.2e10 : 8e9) || (a->starts && rows_groups > MOST_GROUPS));
     a->row_tiles = a->prompt ? prompt_row_tiles((int)head_dim, f32) * WAVES : tiles_of(rows);
     a->blocks = (uint32_t)((rows + 16 * a->row_tiles - 1) / (16 * a->row_tiles));
     a->units = (uint64_t)a->batch * a->blocks;
     if (!a->prompt) {
-        fit_splits(rows_splits((uint64_t)kv_heads * a->units, reach), a->rows, heads, head_dim, max_floats, a);
+        fit_splits(rows_splits((uint64_t)kv_heads * a->units, reach), a->rows, kv_heads, heads, head_dim, max_floats,
+                   a);
         return false;
     }
     const uint64_t others = a->rows > a->max_tokens ? a->rows - a->max_tokens : 0;  // tokens beside the longest's
@@ -431,8 +444,8 @@ bool plan_attention(uint32_t head_dim, uint32_t kv_heads, uint32_t f32, uint64_t
         few->row_tiles = 1;  // most bring one token
         few->blocks = (few_tokens * a->group + 15) / 16;
         few->units = (uint64_t)few->batch * few->blocks;
-        fit_splits(rows_splits((uint64_t)a->batch * kv_heads, reach), (uint64_t)a->batch * few_tokens, heads, head_dim,
-                   max_floats, few);
+        fit_splits(rows_splits((uint64_t)a->batch * kv_heads, reach), (uint64_t)a->batch * few_tokens, kv_heads, heads,
+                   head_dim, max_floats, few);
         max_floats -= few->floats;
     }
     a->units = units_of(*a, a->group, 16 * a->row_tiles);
@@ -450,8 +463,27 @@ bool plan_attention(uint32_t head_dim, uint32_t kv_heads, uint32_t f32, uint64_t
     } else if (head_dim == 256) {
         splits = std::min((640 + busy - 1) / busy, reach / 1024);
     }
-    fit_splits(splits, a->rows, heads, head_dim, max_floats, a);
+    fit_splits(splits, a->rows, kv_heads, heads, head_dim, max_floats, a);
     return both;
+}
+
+// The plans of a call by themselves, on the host: for each {prompt kernel, splits, its workgroups, the
+// join's (0 without one), floats of workspace, most tokens of its sequences}. Returns how many.
+extern "C" int nuq_attention_plan(uint32_t head_dim, uint32_t kv_heads, uint32_t heads, uint32_t f32, uint32_t rows,
+                                  uint32_t batch, uint32_t max_tokens, int ragged, uint64_t max_length, uint32_t window,
+                                  uint64_t max_floats, uint64_t out[12]) {
+    static const int32_t some = 0;
+    AttentionArgs plans[2] = {};
+    plans[0].rows = rows, plans[0].batch = batch, plans[0].max_tokens = max_tokens, plans[0].window = window;
+    plans[0].group = heads / kv_heads, plans[0].starts = ragged ? &some : nullptr;
+    const int count = 1 + plan_attention(head_dim, kv_heads, f32, max_length, heads, max_floats, &plans[0], &plans[1]);
+    for (int i = 0; i < count; ++i) {
+        const AttentionArgs &a = plans[i];
+        const uint64_t v[6] = {a.prompt, a.splits, kv_heads * a.splits * a.units,
+                               a.splits > 1 ? join_groups(a, heads, head_dim, a.splits) : 0, a.floats, a.upto};
+        std::copy(v, v + 6, out + 6 * i);
+    }
+    return count;
 }
 
 hipError_t launch_attention(hipStream_t s, const CacheView &c, uint32_t bits, uint32_t head_dim, uint32_t f32,
@@ -464,8 +496,8 @@ hipError_t launch_attention(hipStream_t s, const CacheView &c, uint32_t bits, ui
                          : f32    ? rows_dispatch<true>(s, c, bits, head_dim, a)
                                   : rows_dispatch<false>(s, c, bits, head_dim, a);
     if (e != hipSuccess || a.splits == 1) return e;
-    const bool few_splits = a.splits <= 8;
-    const uint32_t grid = (uint32_t)units_of(a, heads, few_splits ? 1024 / head_dim : 1);
+    const bool few_splits = a.splits <= FEW_SPLITS;
+    const uint32_t grid = (uint32_t)join_groups(a, heads, head_dim, a.splits);
 #define NUQ_CASE(D)                                                                             \
     if (head_dim == D) {                                                                        \
         if (few_splits && f32) attention_join_rows_kernel<D, true><<<grid, 256, 0, s>>>(a, heads); \

@@ -52,3 +52,30 @@ def test_rows_before_the_end_of_the_queries_keep_their_positions(backend, prompt
     # a count past any the sequence can hold: every row stands before its start
     got = c.run(backend, q=q, starts=np.array([0, 30, 2**31 - 1]), max_tokens=40)
     assert not got[30:].any()
+
+
+def in_long_context(c, tokens):
+    """The case's page table with entries for so many tokens, as one sized for a model's longest context."""
+    table = np.full((len(c.held), max(tokens // c.page, c.table.shape[1])), -1, np.int32)
+    table[:, :c.table.shape[1]] = c.table
+    return table
+
+
+@pytest.mark.parametrize("heads,tokens,batch,context", [(32, 2048, 256, 16384), (64, 2048, 128, 8192), (48, 1000, 400, 16384)])
+def test_a_chunk_among_many_single_tokens_of_long_contexts(backend, heads, tokens, batch, context):
+    """Both plans of the call split their axes."""
+    print(f"[attention] chunk of {tokens} among {batch} sequences, {heads} heads, context {context}", flush=True)
+    rng = np.random.default_rng(28)
+    held = [tokens + 70] + [int(n) for n in rng.integers(1, 40, batch - 1)]
+    c = Case(held, [tokens] + [1] * (batch - 1), kv=8, group=heads // 8, dtype="f16", seed=29)
+    got = c.run(backend, table=in_long_context(c, context), max_tokens=tokens, max_length=context)
+    c.check(got, rows=[0, 1, 63, 64, 500, tokens - 2, tokens - 1])
+
+
+@pytest.mark.parametrize("dtype,heads,batch,context", [("f16", 64, 512, 8192), ("f32", 48, 600, 4096)])
+def test_single_tokens_with_starts_and_no_bound(backend, dtype, heads, batch, context):
+    print(f"[attention] {batch} single tokens with starts, {heads} heads, context {context} {dtype}", flush=True)
+    held = [int(n) for n in np.random.default_rng(30).integers(0, 30, batch)]
+    held[7] = 900
+    c = Case(held, [1] * batch, kv=8, group=heads // 8, dtype=dtype, seed=31)
+    c.check(c.run(backend, table=in_long_context(c, context), starts=np.arange(batch + 1)))
