@@ -854,10 +854,10 @@ int nuq_cache_attention(nuq_context *ctx, const nuq_cache *cache, const nuq_atte
     // rows and positions are ints in the kernels
     if (n.rows > 0x7fffffffull / n.q_heads || n.batch > 0x7fffffffu || n.max_tokens > n.rows)
         return fail(ctx, NUQ_INVALID_SHAPE, "rows, batch or max_tokens out of range");
-    if (n.rows == 0 || n.batch == 0 || n.max_tokens == 0) return NUQ_OK;
     if (!n.starts && n.rows != (uint64_t)n.batch * n.max_tokens)
         return fail(ctx, NUQ_INVALID_SHAPE, "%llu rows are not %u sequences of %u", (unsigned long long)n.rows, n.batch,
                     n.max_tokens);
+    if (n.rows == 0 || n.batch == 0 || n.max_tokens == 0) return NUQ_OK;
     if (n.table_width == 0 || n.table_width > (1ull << 30) / cache->page_tokens || n.table_stride > (1ull << 30) ||
         (n.table_stride < n.table_width && n.batch > 1))
         return fail(ctx, NUQ_INVALID_SHAPE, "page table of width %llu, stride %llu", (unsigned long long)n.table_width,

@@ -79,3 +79,22 @@ def test_single_tokens_with_starts_and_no_bound(backend, dtype, heads, batch, co
     held[7] = 900
     c = Case(held, [1] * batch, kv=8, group=heads // 8, dtype=dtype, seed=31)
     c.check(c.run(backend, table=in_long_context(c, context), starts=np.arange(batch + 1)))
+
+
+def test_rows_that_are_not_whole_sequences_are_refused(backend):
+    """Without starts every sequence brings the same count: fewer rows than sequences, a count of none, or no
+    sequences at all leave rows over."""
+    import torch
+    c = Case([20, 20, 20, 20], [1] * 4, kv=1, group=2, d=64, page=16, seed=32)
+    q, table, lengths = to_gpu(c.q), to_gpu(c.table), to_gpu(np.array(c.held, np.int32))
+    out = torch.full(q.shape, 7.0, device="cuda")
+    for rows, batch, more in ((3, 4, {}), (4, 4, dict(max_tokens=0)), (4, 0, {}), (2, 0, dict(max_tokens=1))):
+        with pytest.raises(nq.InvalidShape):
+            backend.cache_attention(c.cache, q[:rows], out[:rows], table[:batch], lengths[:batch], **more)
+    backend.sync()
+    assert bool((out == 7.0).all())
+    backend.cache_attention(c.cache, q[:0], out[:0], table, lengths)  # no rows: nothing to do
+    starts = to_gpu(np.arange(5, dtype=np.int32))
+    backend.cache_attention(c.cache, q, out, table, lengths, starts=starts, max_tokens=0)  # no row below the bound
+    backend.sync()
+    assert bool((out == 7.0).all())
