@@ -274,7 +274,8 @@ typedef struct nuq_attention {
     const int32_t *lengths;     /* device [batch] */
     const int32_t *starts;      /* device [batch + 1], or null */
     uint32_t batch;
-    uint32_t max_tokens;        /* most new tokens of a sequence; rows past it are not computed, and those
+    uint32_t max_tokens;        /* most new tokens of a sequence, with starts any bound on them (more than
+                                 * `rows` too); rows past it are not computed, and those
                                  * before it keep their positions, lengths[b] - (starts[b + 1] - starts[b]) on */
     uint64_t max_length;        /* most tokens a sequence holds, for the split of the work; 0: the table's */
     float scale;                /* of the scores: positive and finite */

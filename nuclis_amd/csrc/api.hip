@@ -852,8 +852,8 @@ int nuq_cache_attention(nuq_context *ctx, const nuq_cache *cache, const nuq_atte
         return fail(ctx, NUQ_INVALID_SHAPE, "the scale must be finite and positive");
     const uint64_t width = (uint64_t)n.q_heads * cache->head_dim;
     // rows and positions are ints in the kernels
-    if (n.rows > 0x7fffffffull / n.q_heads || n.batch > 0x7fffffffu || n.max_tokens > n.rows)
-        return fail(ctx, NUQ_INVALID_SHAPE, "rows, batch or max_tokens out of range");
+    if (n.rows > 0x7fffffffull / n.q_heads || n.batch > 0x7fffffffu)
+        return fail(ctx, NUQ_INVALID_SHAPE, "rows or batch out of range");
     if (!n.starts && n.rows != (uint64_t)n.batch * n.max_tokens)
         return fail(ctx, NUQ_INVALID_SHAPE, "%llu rows are not %u sequences of %u", (unsigned long long)n.rows, n.batch,
                     n.max_tokens);
@@ -870,7 +870,8 @@ int nuq_cache_attention(nuq_context *ctx, const nuq_cache *cache, const nuq_atte
     nuq::AttentionArgs a{};
     a.q = n.q, a.out = n.out, a.q_stride = n.q_stride, a.out_stride = n.out_stride;
     a.table = n.page_table, a.lengths = n.lengths, a.starts = n.starts, a.table_stride = n.table_stride;
-    a.rows = (uint32_t)n.rows, a.batch = n.batch, a.max_tokens = n.max_tokens, a.group = n.q_heads / cache->kv_heads;
+    a.rows = (uint32_t)n.rows, a.batch = n.batch, a.group = n.q_heads / cache->kv_heads;
+    a.max_tokens = (uint32_t)std::min<uint64_t>(n.max_tokens, n.rows);  // no sequence has more
     a.capacity = (uint32_t)(n.table_width * cache->page_tokens);
     a.window = n.window >= a.capacity ? 0 : n.window;
     a.scale = n.scale * 1.44269504088896340736f;

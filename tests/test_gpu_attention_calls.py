@@ -98,3 +98,15 @@ def test_rows_that_are_not_whole_sequences_are_refused(backend):
     backend.cache_attention(c.cache, q, out, table, lengths, starts=starts, max_tokens=0)  # no row below the bound
     backend.sync()
     assert bool((out == 7.0).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_a_bound_above_the_rows_there_are(backend, dtype):
+    """A constant bound, as a caller keeps for its steps, on a step that brings less."""
+    c = Case([300, 41, 17], [3, 1, 1], kv=2, group=3, dtype=dtype, page=16, seed=33)
+    want = c.run(backend)
+    c.check(want)
+    for bound in (5, 8, 100, 2**32 - 1):
+        assert np.array_equal(c.run(backend, max_tokens=bound), want)
+    long = Case([700, 800], [100, 90], kv=1, group=4, dtype=dtype, page=16, seed=34)
+    long.check(long.run(backend, max_tokens=4096, table=prompt_table(long)))
