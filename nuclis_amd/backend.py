@@ -257,7 +257,7 @@ class KVCache:
                                 device=f"cuda:{device}")
         elif not bytes.is_contiguous():
             raise InvalidShape("InvalidShape: the cache's bytes are not contiguous")
-        self.bytes = bytes
+        self.bytes, self.device = bytes, bytes.get_device()
         self._ref = ctypes.byref(_Cache(bits, page_tokens, kv_heads, head_dim, pages, bytes.data_ptr(),
                                         bytes.numel() * bytes.element_size()))
 
@@ -395,10 +395,16 @@ class Backend:
                     values.cpu().tolist()[:k], total, not bool(flags.cpu().any()))
 
     # -- the quantised cache and the attention over it ------------------------
-    # (shapes, strides and dtypes are asked for once each: a decode step makes
-    # these calls for every layer, and each question to a tensor is 0.1 us)
+    # (shapes, strides, dtypes and devices are asked for once each: a decode step
+    # makes these calls for every layer, and each question to a tensor is 0.1 us;
+    # an address of the host's would fault the GPU)
+    def _elsewhere(self, t, name: str) -> InvalidArgument:
+        return InvalidArgument(f"{name} is on {t.device}, not cuda:{self.device}")
+
     def _index(self, t, dtype, name: str):
-        """The address of a contiguous tensor of this dtype."""
+        """The address of a contiguous tensor of this dtype on this device."""
+        if t.get_device() != self.device:
+            raise self._elsewhere(t, name)
         if t.dtype is not dtype:
             raise InvalidArgument(f"{name} must be {dtype}, not {t.dtype}")
         if not t.is_contiguous():
@@ -406,8 +412,10 @@ class Backend:
         return t.data_ptr()
 
     def _heads(self, t, head_dim: int, name: str):
-        """Checks [rows][heads][head_dim] with contiguous rows: (rows, heads, elements from a row to the
-        next, the dtype's code)."""
+        """Checks [rows][heads][head_dim] with contiguous rows on this device: (rows, heads, elements from a
+        row to the next, the dtype's code)."""
+        if t.get_device() != self.device:
+            raise self._elsewhere(t, name)
         shape, stride = t.shape, t.stride()
         if len(shape) != 3 or shape[2] != head_dim:
             raise InvalidShape(f"InvalidShape: {name} is {tuple(shape)}, not [rows][heads][{head_dim}]")
@@ -418,6 +426,11 @@ class Backend:
         if code is None:
             raise InvalidArgument(f"{name} is {t.dtype}, not float32 or float16")
         return rows, heads, stride[0], code
+
+    def _cache(self, cache: KVCache):
+        if cache.device != self.device:
+            raise self._elsewhere(cache.bytes, "the cache")
+        return cache._ref
 
     def _slots(self, cache: KVCache, k, v, slots):
         tokens, heads, k_stride, code = self._heads(k, cache.head_dim, "k")
@@ -434,12 +447,13 @@ class Backend:
         """Quantises tokens' keys and values [tokens][kv_heads][head_dim] (F32
         or F16; rows may be strided) into their slots (int64; -1 skips)."""
         code, tokens, k_stride, v_stride, at = self._slots(cache, k, v, slots)
-        self._call(_lib.nuq_cache_write, cache._ref, k.data_ptr(), v.data_ptr(), code, k_stride, v_stride, at, tokens)
+        self._call(_lib.nuq_cache_write, self._cache(cache), k.data_ptr(), v.data_ptr(), code, k_stride, v_stride, at, tokens)
 
     def cache_read(self, cache: KVCache, slots, k, v) -> None:
         """Reads slots back into k and v (F32 or F16, both exact)."""
         code, tokens, k_stride, v_stride, at = self._slots(cache, k, v, slots)
-        self._call(_lib.nuq_cache_read, cache._ref, at, tokens, code, k.data_ptr(), v.data_ptr(), k_stride, v_stride)
+        self._call(_lib.nuq_cache_read, self._cache(cache), at, tokens, code, k.data_ptr(), v.data_ptr(), k_stride,
+                   v_stride)
 
     def cache_attention(self, cache: KVCache, q, output, page_table, lengths, starts=None, scale: float | None = None,
                         window: int = 0, max_tokens: int | None = None, max_length: int = 0) -> None:
@@ -458,6 +472,8 @@ class Backend:
         table, table_stride = page_table.shape, page_table.stride()
         if len(table) != 2 or table[0] != batch:
             raise InvalidShape(f"InvalidShape: page table {tuple(table)} for {batch} sequences")
+        if page_table.get_device() != self.device:
+            raise self._elsewhere(page_table, "the page table")
         if page_table.dtype is not int32 or table_stride[1] != 1:
             raise InvalidArgument("the page table is not int32 with contiguous rows")
         first = None
@@ -473,7 +489,7 @@ class Backend:
                           page_table.data_ptr(), table_stride[0], table[1], self._index(lengths, int32, "lengths"),
                           first, batch, max_tokens, max_length, cache.head_dim ** -0.5 if scale is None else scale,
                           window)
-        self._call(_lib.nuq_cache_attention, cache._ref, ctypes.byref(args))
+        self._call(_lib.nuq_cache_attention, self._cache(cache), ctypes.byref(args))
 
     def logprobs(self, logits, targets, logprobs, entropy, top_ids=None, top_logprobs=None) -> None:
         """Log probabilities of given tokens (nuq_logprobs, include/nuq.h):
@@ -481,6 +497,8 @@ class Backend:
         [rows]; logprobs and entropy F32 [rows]; top_ids int32 and top_logprobs F32
         [rows][top], the most probable tokens (both or neither)."""
         torch = self._torch
+        if logits.get_device() != self.device:
+            raise self._elsewhere(logits, "the logits")
         shape, stride = logits.shape, logits.stride()
         if len(shape) != 2 or (stride[1] != 1 and shape[1] > 1):
             raise InvalidShape(f"InvalidShape: logits {tuple(shape)} are not contiguous rows")
