@@ -68,6 +68,16 @@ class CachedLayer:
             self.lengths[b] += count
         return np.concatenate(slots)
 
+    def _shrink(self, lengths) -> None:
+        """Takes a step back: the sequences hold `lengths` tokens again, and the pages past them are free, in
+        the order they were in."""
+        for b in reversed(range(len(lengths))):
+            keep = -(-lengths[b] // self.cache.page_tokens)
+            while len(self.pages[b]) > keep:
+                self.free.append(self.pages[b].pop())
+                self.table[b, len(self.pages[b])] = -1
+            self.lengths[b] = lengths[b]
+
     def _device(self, array):
         return self._torch.from_numpy(np.ascontiguousarray(array)).to(f"cuda:{self.backend.device}")
 
@@ -77,15 +87,23 @@ class CachedLayer:
     def forward(self, x, counts):
         """x [sum(counts)][hidden] F32: every sequence's new tokens (counts[b], 0 for a
         sequence that rests), one sequence's behind the other's. Returns the
-        logits [sum(counts)][vocabulary], good until the next call."""
-        torch, b, m = self._torch, self.backend, self.mats
+        logits [sum(counts)][vocabulary], good until the next call. If it raises, the sequences hold
+        what they held before."""
         rows = int(sum(counts))
         if len(counts) != len(self.lengths) or min(counts, default=0) < 0 or tuple(x.shape) != (rows, self.hidden):
             raise nb.InvalidShape(f"InvalidShape: {len(counts)} counts of {len(self.lengths)} sequences, "
                                   f"{rows} rows, x {tuple(x.shape)}")
         if rows == 0:
-            return self._buffer("logits", 0, m["lm_head"].rows)
-        slots = self._device(self._grow(counts))
+            return self._buffer("logits", 0, self.mats["lm_head"].rows)
+        before = list(self.lengths)
+        try:
+            return self._step(x, counts, rows, self._device(self._grow(counts)))
+        except BaseException:
+            self._shrink(before)  # a step that failed has not happened: it can be tried again
+            raise
+
+    def _step(self, x, counts, rows: int, slots):
+        torch, b, m = self._torch, self.backend, self.mats
         q_rows, kv_rows, single = self.q_rows, self.kv_rows, rows == 1
         qkv = self._buffer("qkv", rows, q_rows + 2 * kv_rows)
         q, k, v = qkv[:, :q_rows], qkv[:, q_rows:q_rows + kv_rows], qkv[:, q_rows + kv_rows:]
