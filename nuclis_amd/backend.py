@@ -138,6 +138,9 @@ def lib() -> ctypes.CDLL:
     if _lib is None:
         if not LIB_PATH.exists():
             raise RuntimeError(f"{LIB_PATH} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'`")
+        # torch first: the library then binds to the HIP runtime that torch ships. The other way round the
+        # process holds two of them, and whichever comes second finds no device.
+        import torch  # noqa: F401
         L = ctypes.CDLL(str(LIB_PATH))
         vp, u32, u64 = ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint64
         mp = ctypes.POINTER(_Matrix)
