@@ -85,7 +85,7 @@ class CachedLayer:
         self.backend.matmul(self.mats[name], x, x.stride(0), out, out.stride(0), x.shape[0])
 
     def forward(self, x, counts):
-        """x [sum(counts)][hidden] F32: every sequence's new tokens (counts[b], 0 for a
+        """x [sum(counts)][hidden] F32, rows contiguous: every sequence's new tokens (counts[b], 0 for a
         sequence that rests), one sequence's behind the other's. Returns the
         logits [sum(counts)][vocabulary], good until the next call. If it raises, the sequences hold
         what they held before."""
@@ -93,6 +93,10 @@ class CachedLayer:
         if len(counts) != len(self.lengths) or min(counts, default=0) < 0 or tuple(x.shape) != (rows, self.hidden):
             raise nb.InvalidShape(f"InvalidShape: {len(counts)} counts of {len(self.lengths)} sequences, "
                                   f"{rows} rows, x {tuple(x.shape)}")
+        if x.dtype is not self._torch.float32 or x.get_device() != self.backend.device:
+            raise nb.InvalidArgument(f"x is {x.dtype} on {x.device}, not float32 on cuda:{self.backend.device}")
+        if self.hidden > 1 and x.stride(1) != 1:
+            raise nb.InvalidShape(f"InvalidShape: x's rows are not contiguous (strides {x.stride()})")
         if rows == 0:
             return self._buffer("logits", 0, self.mats["lm_head"].rows)
         before = list(self.lengths)
