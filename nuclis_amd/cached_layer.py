@@ -32,6 +32,16 @@ class CachedLayer:
         import torch
         self._torch, self.backend, self.mats, self.window = torch, backend, mats, window
         self.q_rows, self.kv_rows, self.hidden = mats["q"].rows, mats["k"].rows, mats["q"].columns
+        ffn = mats["gate"].rows
+        fit = {"q": (self.q_rows, self.hidden), "k": (self.kv_rows, self.hidden), "v": (self.kv_rows, self.hidden),
+               "o": (self.hidden, self.q_rows), "gate": (ffn, self.hidden), "up": (ffn, self.hidden),
+               "down": (self.hidden, ffn), "lm_head": (mats["lm_head"].rows, self.hidden)}
+        for name, (rows, columns) in fit.items():
+            if (mats[name].rows, mats[name].columns) != (rows, columns):
+                raise nb.InvalidShape(f"InvalidShape: {name} is {mats[name].rows} x {mats[name].columns}, "
+                                      f"not {rows} x {columns}")
+        if self.kv_rows % head_dim or self.q_rows % self.kv_rows:
+            raise nb.InvalidShape(f"InvalidShape: {self.q_rows} and {self.kv_rows} rows are not whole heads of {head_dim}")
         self.head_dim = head_dim
         self.cache = nb.KVCache(bits, pages, page_tokens, self.kv_rows // head_dim, head_dim, device=backend.device)
         self.lengths = [0] * sequences

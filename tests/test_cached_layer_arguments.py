@@ -38,3 +38,18 @@ def test_inputs(layer, rows):
     assert layer.ran == [] and layer.lengths == [0, 0]
     layer.forward(OnGpu(rows, 64), counts)
     assert layer.ran == [counts]
+
+
+def test_matrices_that_do_not_fit_each_other():
+    """A v of more rows than k would be written past its place in the merged row; heads that are not whole
+    have no place in the cache."""
+    good = {"q": (384, 64), "k": (128, 64), "v": (128, 64), "o": (64, 384), "gate": (192, 64), "up": (192, 64),
+            "down": (64, 192), "lm_head": (1000, 64)}
+    changes = [{n: s} for n, s in (("v", (192, 64)), ("v", (64, 64)), ("k", (96, 64)), ("q", (320, 64)), ("o", (64, 320)),
+                                   ("o", (128, 384)), ("up", (256, 64)), ("gate", (192, 32)), ("down", (64, 128)),
+                                   ("lm_head", (1000, 128)))]
+    changes += [{"k": (64, 64)}, {"k": (96, 64), "v": (96, 64)}, {"q": (320, 64), "o": (64, 320)}]
+    for change in changes:
+        mats = {n: SimpleNamespace(rows=r, columns=c) for n, (r, c) in {**good, **change}.items()}
+        with pytest.raises(nq.InvalidShape):
+            CachedLayer(SimpleNamespace(device="none"), mats, sequences=2, pages=4, head_dim=64)
