@@ -13,7 +13,8 @@ them and decoded tokens of several sequences in one step:
 
 All projections, the cache and the attention run in libnuq.so; torch holds the
 buffers and adds. Pages are handed out as sequences grow and come back with
-`release`; the host keeps the lengths, so a step asks the GPU nothing.
+`release`; the host keeps the lengths, so a step asks the GPU nothing and waits for
+nothing: steps queue behind each other (but where a buffer or the workspace grows).
 """
 from __future__ import annotations
 
@@ -89,7 +90,14 @@ class CachedLayer:
             self.lengths[b] = lengths[b]
 
     def _device(self, array):
-        return self._torch.from_numpy(np.ascontiguousarray(array)).to(f"cuda:{self.backend.device}")
+        """The array on the GPU, by a copy that is queued: from pageable memory it would wait for all work
+        before it. (Pinned blocks come from torch's pool, which keeps them until their copy is done.)"""
+        torch = self._torch
+        if torch.cuda.is_current_stream_capturing():
+            raise nb.InvalidArgument("a step's tables and lengths come from the host: a graph would replay this step's")
+        array = torch.from_numpy(np.ascontiguousarray(array))
+        held = torch.empty(array.shape, dtype=array.dtype, pin_memory=True)
+        return held.copy_(array).to(f"cuda:{self.backend.device}", non_blocking=True)
 
     def _project(self, name: str, x, out) -> None:
         self.backend.matmul(self.mats[name], x, x.stride(0), out, out.stride(0), x.shape[0])

@@ -47,3 +47,54 @@ def test_a_step_that_fails_can_be_tried_again(monkeypatch, fails):
         assert bool((got == want).all())
         assert same(state_of(tried), state_of(plain))
     b.close()
+
+
+def test_steps_do_not_wait_for_the_gpu():
+    """Once its buffers stand a step makes no call that torch knows to wait for the stream, and results
+    of steps queued behind each other are those of steps that are waited for."""
+    _, mats = build()
+    b = nq.Backend(0)
+    queued, waited = (CachedLayer(b, mats, sequences=3, pages=24, page_tokens=16, head_dim=D) for _ in range(2))
+    rng = np.random.default_rng(41)
+    steps = [([30, 40, 10], to_gpu(rng.standard_normal((80, HIDDEN)).astype(np.float32)))]
+    for _ in range(6):
+        steps.append(([1, 1, 1], to_gpu(rng.standard_normal((3, HIDDEN)).astype(np.float32))))
+        steps.append(([1, 0, 4], to_gpu(rng.standard_normal((5, HIDDEN)).astype(np.float32))))
+    want = []
+    for counts, x in steps:
+        want.append(waited.forward(x, counts).clone())
+        b.sync()
+    got = [queued.forward(steps[0][1], steps[0][0]).clone()]
+    b.sync()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        got += [queued.forward(x, counts).clone() for counts, x in steps[1:]]
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    b.sync()
+    for g, w in zip(got, want):
+        assert bool((g == w).all())
+    b.close()
+
+
+def test_a_step_is_not_captured():
+    """A graph would hold copies from host memory that another step has by then."""
+    _, mats = build()
+    b = nq.Backend(0)
+    layer = CachedLayer(b, mats, sequences=1, pages=4, page_tokens=16, head_dim=D)
+    x = to_gpu(np.random.default_rng(42).standard_normal((1, HIDDEN)).astype(np.float32))
+    layer.forward(x, [1])
+    b.sync()
+    before = state_of(layer)
+    other = torch.zeros(4, device="cuda")
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.stream(stream), torch.cuda.graph(graph, stream=stream):
+        other += 1
+        with pytest.raises(nq.InvalidArgument):
+            layer.forward(x, [1])
+    assert same(state_of(layer), before)
+    graph.replay()
+    layer.forward(x, [1])
+    b.sync()
+    assert layer.lengths == [2] and bool((other == 1).all())
+    b.close()
