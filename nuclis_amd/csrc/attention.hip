@@ -384,7 +384,6 @@ static void fit_splits(uint64_t splits, uint64_t rows, uint32_t kv_heads, uint32
     splits = std::min<uint64_t>(std::min<uint64_t>(splits, MAX_SPLITS), MOST_GROUPS / (kv_heads * a->units));
     splits = std::max<uint64_t>(1, splits);
     const uint64_t each = rows * heads * (head_dim + 2);
-    max_floats = std::min<uint64_t>(max_floats, 1ull << 26);  // 256 MiB of partial results
     if (splits > 1 && splits * each > max_floats) splits = std::max<uint64_t>(1, max_floats / each);
     if (splits > 1 && join_groups(*a, heads, head_dim, splits) > MOST_GROUPS) splits = 1;
     a->splits = (uint32_t)splits;
@@ -416,6 +415,7 @@ static void fit_splits(uint64_t splits, uint64_t rows, uint32_t kv_heads, uint32
 // by the prompt kernel 738; calls of their own, which know each other's lengths, 78).
 bool plan_attention(uint32_t head_dim, uint32_t kv_heads, uint32_t f32, uint64_t max_length, uint32_t heads,
                     uint64_t max_floats, AttentionArgs *a, AttentionArgs *few) {
+    max_floats = std::min<uint64_t>(max_floats, 1ull << 26);  // 256 MiB of a call's partial results
     const uint64_t rows = (uint64_t)a->max_tokens * a->group;
     uint64_t reach = max_length;  // tokens the last row and those before it may see
     if (a->window) reach = std::min<uint64_t>(reach, (uint64_t)a->window + a->max_tokens);

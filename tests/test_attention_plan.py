@@ -66,3 +66,19 @@ def test_plans_stay_within_a_launch():
         found = plans(*where)
         check(found, where)
         assert sum(p["floats"] for p in found) <= floats, (where, found)
+
+
+def test_partial_results_of_a_call_stay_within_256_mib():
+    """Both plans' together: a long chunk with wide heads among single tokens whose axes are split too."""
+    found = plans(256, 1, 16, 0, 2055, 8, 2048, 1, 1 << 18)
+    assert len(found) == 2 and all(p["splits"] > 1 for p in found)
+    rng = random.Random(8)
+    both = 0
+    for _ in range(20000):
+        kv, group, d = rng.choice([1, 1, 2, 4]), rng.choice([4, 8, 16]), rng.choice([64, 128, 256])
+        batch, most = rng.randint(2, 12), rng.randint(300, 4000)
+        found = plans(d, kv, kv * group, rng.randint(0, 1), most + batch - 1, batch, most, 1,
+                      rng.choice([1 << 14, 1 << 16, 1 << 18]))
+        both += len(found) == 2 and all(p["splits"] > 1 for p in found)
+        assert 4 * sum(p["floats"] for p in found) <= 256 << 20, (kv, group, d, batch, most, found)
+    assert both > 1000
