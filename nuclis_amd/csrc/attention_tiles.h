@@ -355,7 +355,13 @@ template <int BITS, int D, int RT, bool F32> struct Rows {
 #pragma unroll
                 for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) asm volatile("" : "+v"(q[0][t][g].w[e]));
+                    for (int e = 0; e < 4; ++e) {
+                        // infinities become NaN, as the parts of an F32 query do: scores of -inf would
+                        // make the row one that sees nothing
+                        const half2v x = as_half2(q[0][t][g].w[e]);
+                        q[0][t][g].w[e] = as_u32(x * (_Float16)0.0f + x);
+                        asm volatile("" : "+v"(q[0][t][g].w[e]));
+                    }
             } else {
                 float most = 0.0f;
 #pragma unroll

@@ -110,3 +110,23 @@ def test_a_bound_above_the_rows_there_are(backend, dtype):
         assert np.array_equal(c.run(backend, max_tokens=bound), want)
     long = Case([700, 800], [100, 90], kv=1, group=4, dtype=dtype, page=16, seed=34)
     long.check(long.run(backend, max_tokens=4096, table=prompt_table(long)))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
+@pytest.mark.parametrize("tokens,length", [(1, 1), (3, 3), (3, 700), (70, 90)])
+def test_queries_that_are_not_finite(backend, dtype, value, tokens, length):
+    """NaN for the rows and heads that hold one, whatever the signs of the scores; zeros where such a row
+    sees nothing; the others untouched."""
+    c = Case([length, 0], [tokens, tokens], kv=2, group=2, d=64, page=16, dtype=dtype, seed=35)
+    kw = dict(table=prompt_table(c)) if tokens * c.group > 64 else {}
+    want = c.run(backend, **kw)
+    c.check(want)
+    hit = np.zeros((2 * tokens, 4), bool)
+    for row, head, dim in ((0, 0, 0), (0, 3, 63), (tokens - 1, 1, 20), (tokens, 2, 7)):
+        c.q[row, head, dim] = value
+        hit[row, head] = row < tokens
+    got = c.run(backend, **kw)
+    assert np.array_equal(np.isnan(got).all(-1), hit) and np.array_equal(np.isnan(got).any(-1), hit)
+    assert np.array_equal(got[~hit], want[~hit])
+    assert not got[tokens:].any()
