@@ -880,7 +880,8 @@ int nuq_cache_attention(nuq_context *ctx, const nuq_cache *cache, const nuq_atte
     nuq::AttentionArgs few{};
     bool both = false;
     const auto plan_with = [&](uint64_t floats) {
-        both = nuq::plan_attention(cache->head_dim, cache->kv_heads, f32, longest, n.q_heads, floats, &a, &few);
+        both = nuq::plan_attention(cache->head_dim, cache->kv_heads, f32, longest, n.q_heads, floats, nuq::compute_units(), &a,
+                                   &few);
     };
     plan_with(UINT64_MAX);
     // without the workspace it wants (a capture, no memory): fewer splits
@@ -918,11 +919,12 @@ int nuq_logprobs(nuq_context *ctx, const void *logits, uint32_t dtype, uint64_t 
     if ((uintptr_t)logits % (dtype == NUQ_F16 ? 2 : 4) ||
         ((uintptr_t)targets | (uintptr_t)logprobs | (uintptr_t)entropy | (uintptr_t)top_ids | (uintptr_t)top_logprobs) % 4)
         return fail(ctx, NUQ_INVALID_SHAPE, "misaligned logits, targets or results");
-    (void)ensure_workspace(ctx, nuq::logprobs_floats((uint32_t)rows, (uint32_t)count, top));
+    const uint32_t cus = nuq::compute_units();
+    (void)ensure_workspace(ctx, nuq::logprobs_floats((uint32_t)rows, (uint32_t)count, top, cus));
     return hip_check(ctx,
                      nuq::launch_logprobs(ctx->stream, logits, dtype == NUQ_F16, (uint32_t)rows, (uint32_t)count, stride,
                                           targets, top, logprobs, entropy, top_ids, top_logprobs, ctx->split.work,
-                                          (uint64_t)ctx->split.tiles * 256 * 256),
+                                          (uint64_t)ctx->split.tiles * 256 * 256, cus),
                      "log probabilities launch");
 }
 

@@ -41,10 +41,10 @@ hipError_t launch_attention_prompt(hipStream_t s, const CacheView &c, uint32_t b
 constexpr uint64_t MOST_GROUPS = 0x00ffffffull;
 
 // Fills in the plan of a call: row tiles of 16, blocks of them, splits of the
-// long axis with at most `max_floats` of workspace. Returns whether sequences of few new
+// long axis with at most `max_floats` of workspace, for `cus` compute units. Returns whether sequences of few new
 // tokens are a plan of their own, `few`, beside those of many in `a`.
 bool plan_attention(uint32_t head_dim, uint32_t kv_heads, uint32_t f32, uint64_t max_length, uint32_t heads,
-                    uint64_t max_floats, AttentionArgs *a, AttentionArgs *few);
+                    uint64_t max_floats, uint32_t cus, AttentionArgs *a, AttentionArgs *few);
 hipError_t launch_attention(hipStream_t s, const CacheView &c, uint32_t bits, uint32_t head_dim, uint32_t f32,
                             uint32_t heads, AttentionArgs a, float *work);
 

@@ -367,9 +367,9 @@ static uint64_t units_of(const AttentionArgs &a, uint64_t by, uint64_t of) {
     return a.starts ? std::min(all, a.rows * by / of + sequences) : all;
 }
 // The splits of the rows kernel's calls (plan_attention).
-static uint64_t rows_splits(uint64_t groups, uint64_t reach) {
+static uint64_t rows_splits(uint64_t groups, uint64_t reach, uint64_t cus) {
     if (reach <= 512) return 1;
-    return std::max(std::min(256 / groups, (reach + 127) / 128), std::min(1024 / groups, (reach + 1023) / 1024));
+    return std::max(std::min(cus / groups, (reach + 127) / 128), std::min(4 * cus / groups, (reach + 1023) / 1024));
 }
 // Workgroups of the kernel that joins a plan's splits: D / 4 threads a (row, head) where they are
 // few, a workgroup each where they are many.
@@ -402,8 +402,8 @@ static void fit_splits(uint64_t splits, uint64_t rows, uint32_t kv_heads, uint32
 // us, 7.7 split in three and joined); then 128 tokens each while a workgroup a CU wants
 // work (4096 tokens: 8.1 us, 10.5 at 512 each), and four a CU where each has 1024
 // (batch of 32 up to 16384: 83 us, 88 at two a CU, 114 at one). Prompts: where
-// rows are few against the tokens they see, n that makes the least of (rounds of the 512
-// workgroups that run at once) / n and what joining n costs, 170 n / tokens (300 tokens
+// rows are few against the tokens they see, n that makes the least of (rounds of the workgroups that run
+// at once, two a CU) / n and what joining n costs, 170 n / tokens (300 tokens
 // after 16000, F16, 80 workgroups: 196 us in 3, 156 in 6, 196 in 7; 1000, 256 workgroups: 411 in
 // 2, 424 in 4; a window of 4096 at D = 256, 256 workgroups: 206 in 2, 239 in 4). A prompt from its
 // start on is in balance by itself (2000 tokens: 164 us split, 86 not), but for wide
@@ -414,7 +414,7 @@ static void fit_splits(uint64_t splits, uint64_t rows, uint32_t kv_heads, uint32
 // others by the prompt kernel (a prompt of 512 among 32 single tokens after 8000: 120 us, all
 // by the prompt kernel 738; calls of their own, which know each other's lengths, 78).
 bool plan_attention(uint32_t head_dim, uint32_t kv_heads, uint32_t f32, uint64_t max_length, uint32_t heads,
-                    uint64_t max_floats, AttentionArgs *a, AttentionArgs *few) {
+                    uint64_t max_floats, uint32_t cus, AttentionArgs *a, AttentionArgs *few) {
     max_floats = std::min<uint64_t>(max_floats, 1ull << 26);  // 256 MiB of a call's partial results
     const uint64_t rows = (uint64_t)a->max_tokens * a->group;
     uint64_t reach = max_length;  // tokens the last row and those before it may see
@@ -431,7 +431,7 @@ bool plan_attention(uint32_t head_dim, uint32_t kv_heads, uint32_t f32, uint64_t
     a->blocks = (uint32_t)((rows + 16 * a->row_tiles - 1) / (16 * a->row_tiles));
     a->units = (uint64_t)a->batch * a->blocks;
     if (!a->prompt) {
-        fit_splits(rows_splits((uint64_t)kv_heads * a->units, reach), a->rows, kv_heads, heads, head_dim, max_floats,
+        fit_splits(rows_splits((uint64_t)kv_heads * a->units, reach, cus), a->rows, kv_heads, heads, head_dim, max_floats,
                    a);
         return false;
     }
@@ -444,8 +444,8 @@ bool plan_attention(uint32_t head_dim, uint32_t kv_heads, uint32_t f32, uint64_t
         few->row_tiles = 1;  // most bring one token
         few->blocks = (few_tokens * a->group + 15) / 16;
         few->units = (uint64_t)few->batch * few->blocks;
-        fit_splits(rows_splits((uint64_t)a->batch * kv_heads, reach), (uint64_t)a->batch * few_tokens, kv_heads, heads,
-                   head_dim, max_floats, few);
+        fit_splits(rows_splits((uint64_t)a->batch * kv_heads, reach, cus), (uint64_t)a->batch * few_tokens, kv_heads,
+                   heads, head_dim, max_floats, few);
         max_floats -= few->floats;
     }
     a->units = units_of(*a, a->group, 16 * a->row_tiles);
@@ -457,11 +457,11 @@ bool plan_attention(uint32_t head_dim, uint32_t kv_heads, uint32_t f32, uint64_t
     if (reach >= 4ull * a->max_tokens) {
         double least = 1e30;
         for (uint64_t n = 1; n <= std::max<uint64_t>(1, std::min<uint64_t>(reach / 1024, MAX_SPLITS)); ++n) {
-            const double cost = (double)((busy * n + 511) / 512) / n + 170.0 * n / reach;
+            const double cost = (double)((busy * n + 2 * cus - 1) / (2 * cus)) / n + 170.0 * n / reach;
             if (cost < least) least = cost, splits = n;
         }
     } else if (head_dim == 256) {
-        splits = std::min((640 + busy - 1) / busy, reach / 1024);
+        splits = std::min((cus * 5 / 2 + busy - 1) / busy, reach / 1024);
     }
     fit_splits(splits, a->rows, kv_heads, heads, head_dim, max_floats, a);
     return both;
@@ -471,12 +471,12 @@ bool plan_attention(uint32_t head_dim, uint32_t kv_heads, uint32_t f32, uint64_t
 // join's (0 without one), floats of workspace, most tokens of its sequences}. Returns how many.
 extern "C" int nuq_attention_plan(uint32_t head_dim, uint32_t kv_heads, uint32_t heads, uint32_t f32, uint32_t rows,
                                   uint32_t batch, uint32_t max_tokens, int ragged, uint64_t max_length, uint32_t window,
-                                  uint64_t max_floats, uint64_t out[12]) {
+                                  uint64_t max_floats, uint32_t cus, uint64_t out[12]) {
     static const int32_t some = 0;
     AttentionArgs plans[2] = {};
     plans[0].rows = rows, plans[0].batch = batch, plans[0].max_tokens = max_tokens, plans[0].window = window;
     plans[0].group = heads / kv_heads, plans[0].starts = ragged ? &some : nullptr;
-    const int count = 1 + plan_attention(head_dim, kv_heads, f32, max_length, heads, max_floats, &plans[0], &plans[1]);
+    const int count = 1 + plan_attention(head_dim, kv_heads, f32, max_length, heads, max_floats, cus, &plans[0], &plans[1]);
     for (int i = 0; i < count; ++i) {
         const AttentionArgs &a = plans[i];
         const uint64_t v[6] = {a.prompt, a.splits, kv_heads * a.splits * a.units,

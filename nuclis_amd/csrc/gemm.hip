@@ -849,7 +849,7 @@ __global__ void __launch_bounds__(256) split_reduce_kernel(const float *__restri
     if (m < tokens && n < rows) y[(uint64_t)m * out_stride + n] = v;
 }
 
-static uint32_t compute_units() {
+uint32_t compute_units() {
     static uint32_t cached = 0;
     if (!cached) {
         int dev = 0, n = 0;

@@ -84,13 +84,16 @@ hipError_t launch_penalize(hipStream_t s, float *logits, uint32_t count, const u
 hipError_t launch_topk(hipStream_t s, const float *logits, uint32_t count, uint32_t k, float temperature,
                        uint64_t *scratch, float *values, uint32_t *indices, float *sums, uint32_t *flags);
 
+// Of the device in use, for the planners (gemm.hip).
+uint32_t compute_units();
+
 // Log probabilities of rows of logits (logprobs.hip); `floats` of workspace,
 // without which a row is not split over workgroups.
 constexpr uint32_t LOGPROBS_MAX_TOP = 32;
-uint64_t logprobs_floats(uint32_t rows, uint32_t count, uint32_t top);
+uint64_t logprobs_floats(uint32_t rows, uint32_t count, uint32_t top, uint32_t cus);
 hipError_t launch_logprobs(hipStream_t s, const void *logits, uint32_t f16, uint32_t rows, uint32_t count,
                            uint64_t stride, const int32_t *targets, uint32_t top, float *logprobs, float *entropy,
-                           uint32_t *ids, float *tops, float *work, uint64_t floats);
+                           uint32_t *ids, float *tops, float *work, uint64_t floats, uint32_t cus);
 
 // The quantised cache (cache.hip): tokens into their slots and back.
 uint64_t cache_tile_bytes(uint32_t bits, uint32_t head_dim);

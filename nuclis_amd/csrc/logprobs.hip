@@ -364,26 +364,26 @@ template <typename T> __global__ void __launch_bounds__(THREADS) logprobs_join_k
     finish(a, row, id, target, s, list, n, tid);
 }
 
-uint32_t splits_of(uint32_t rows, uint32_t count) {
+uint32_t splits_of(uint32_t rows, uint32_t count, uint32_t cus) {
     // one step of a workgroup is 4096 logits; four workgroups a CU fill the card
     const uint32_t steps = (count + THREADS * EACH - 1) / (THREADS * EACH);
-    const uint32_t wanted = (1024 + rows - 1) / rows;
+    const uint32_t wanted = (4 * cus + rows - 1) / rows;
     return wanted < steps ? (wanted < 64 ? wanted : 64) : (steps < 64 ? steps : 64);
 }
 
 }  // namespace
 
-uint64_t logprobs_floats(uint32_t rows, uint32_t count, uint32_t top) {
-    const uint64_t splits = splits_of(rows, count);
+uint64_t logprobs_floats(uint32_t rows, uint32_t count, uint32_t top, uint32_t cus) {
+    const uint64_t splits = splits_of(rows, count, cus);
     return splits == 1 ? 0 : rows * splits * (2ull * top + 3);
 }
 
 hipError_t launch_logprobs(hipStream_t s, const void *logits, uint32_t f16, uint32_t rows, uint32_t count,
                            uint64_t stride, const int32_t *targets, uint32_t top, float *logprobs, float *entropy,
-                           uint32_t *ids, float *tops, float *work, uint64_t floats) {
+                           uint32_t *ids, float *tops, float *work, uint64_t floats, uint32_t cus) {
     LogprobArgs a = {logits, stride, targets, logprobs, entropy, ids, tops, rows, count, top, 1, 0, nullptr, nullptr};
-    a.splits = splits_of(rows, count);
-    if (a.splits > 1 && logprobs_floats(rows, count, top) > floats) a.splits = 1;
+    a.splits = splits_of(rows, count, cus);
+    if (a.splits > 1 && logprobs_floats(rows, count, top, cus) > floats) a.splits = 1;
     const uint32_t v = f16 ? 8 : 4, step = THREADS * EACH / v;
     const uint64_t vectors = ((uint64_t)count + v - 1 + v - 1) / v;  // a row may begin inside a vector
     a.span = (uint32_t)((vectors + a.splits - 1) / a.splits + step - 1) / step * step;

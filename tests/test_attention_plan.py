@@ -11,12 +11,12 @@ MOST = 0xffffff  # workgroups of a launch
 FIELDS = ("prompt", "splits", "groups", "join", "floats", "upto")
 
 
-def plans(head_dim, kv_heads, heads, f32, rows, batch, max_tokens, ragged, max_length, window=0, max_floats=1 << 62):
+def plans(head_dim, kv_heads, heads, f32, rows, batch, max_tokens, ragged, max_length, window=0, max_floats=1 << 62, cus=256):
     f = nq.lib().nuq_attention_plan
     u32, u64 = ctypes.c_uint32, ctypes.c_uint64
-    f.argtypes = [u32, u32, u32, u32, u32, u32, u32, ctypes.c_int, u64, u32, u64, u64 * 12]
+    f.argtypes = [u32, u32, u32, u32, u32, u32, u32, ctypes.c_int, u64, u32, u64, u32, u64 * 12]
     out = (u64 * 12)()
-    count = f(head_dim, kv_heads, heads, f32, rows, batch, max_tokens, ragged, max_length, window, max_floats, out)
+    count = f(head_dim, kv_heads, heads, f32, rows, batch, max_tokens, ragged, max_length, window, max_floats, cus, out)
     return [dict(zip(FIELDS, out[6 * i:6 * i + 6])) for i in range(count)]
 
 
@@ -82,3 +82,19 @@ def test_partial_results_of_a_call_stay_within_256_mib():
         both += len(found) == 2 and all(p["splits"] > 1 for p in found)
         assert 4 * sum(p["floats"] for p in found) <= 256 << 20, (kv, group, d, batch, most, found)
     assert both > 1000
+
+
+@pytest.mark.parametrize("heads,rows,batch,tokens,length,f32,many,few", [
+    (48, 1, 1, 1, 4096, 1, 32, 8),         # one token: a workgroup a compute unit
+    (48, 32, 32, 1, 16384, 0, 4, 1),       # single tokens: four
+    (48, 300, 1, 300, 16000, 0, 6, 3),     # a chunk, 80 workgroups: rounds of two
+])
+def test_splits_follow_the_compute_units(heads, rows, batch, tokens, length, f32, many, few):
+    """The shape's splits on a whole device and on a quarter of one."""
+    one = [plans(128, 8, heads, f32, rows, batch, tokens, 0, length, cus=cus)[0]["splits"] for cus in (256, 64)]
+    assert one == [many, few]
+
+
+def test_splits_of_wide_heads_follow_the_compute_units():
+    splits = [plans(256, 4, 16, 0, 4096, 1, 4096, 0, 4096, cus=cus)[0]["splits"] for cus in (256, 64, 1024)]
+    assert splits == [2, 1, 3]  # 512 workgroups; four splits' partial results would not fit
