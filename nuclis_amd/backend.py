@@ -81,8 +81,6 @@ class _TopKBuffers(ctypes.Structure):
                 ("flags", ctypes.c_void_p)]
 
 
-LOGPROBS_MAX_TOP = 32  # NUQ_LOGPROBS_MAX_TOP (include/nuq.h)
-
 # Backend.topk limits (backends/metal/ops/sampling.zig:15-22)
 TOPK_CAPACITY, TOPK_PARTIALS, TOPK_MAX_COUNT = 256, 64, 262144
 

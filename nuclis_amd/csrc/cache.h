@@ -41,8 +41,6 @@
 
 namespace nuq {
 
-constexpr int CACHE_TILE = 16;
-
 template <int BITS, int D> struct CacheGeometry {
     static constexpr int GROUPS = D / 32;
     static constexpr int CHUNK = D * BITS / 32 < 16 ? D * BITS / 32 : 16;  // bytes a lane loads of a unit
@@ -54,7 +52,6 @@ template <int BITS, int D> struct CacheGeometry {
     static constexpr int SCALES = D;               // 16 tokens * D / 32 groups * 2 bytes
     static constexpr int K_SCALES = CODES, V_CODES = CODES + SCALES, V_SCALES = 2 * CODES + SCALES;
     static constexpr int TILE_BYTES = 2 * (CODES + SCALES);
-    static constexpr float MAX_SCALE = BITS == 4 ? 2720.0f : 56.0f;
     static constexpr int OFFSET = BITS == 4 ? 8 : 128;
 };
 

@@ -89,7 +89,6 @@ uint32_t compute_units();
 
 // Log probabilities of rows of logits (logprobs.hip); `floats` of workspace,
 // without which a row is not split over workgroups.
-constexpr uint32_t LOGPROBS_MAX_TOP = 32;
 uint64_t logprobs_floats(uint32_t rows, uint32_t count, uint32_t top, uint32_t cus);
 hipError_t launch_logprobs(hipStream_t s, const void *logits, uint32_t f16, uint32_t rows, uint32_t count,
                            uint64_t stride, const int32_t *targets, uint32_t top, float *logprobs, float *entropy,
