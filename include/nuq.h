@@ -256,8 +256,9 @@ int nuq_cache_read(nuq_context *ctx, const nuq_cache *cache, const int64_t *slot
  * is null. The query at position p sees the cached positions j <= p, with a
  * window also j > p - window. q and out are [rows][q_heads][head_dim] of `dtype`,
  * 16-byte aligned rows; query head i reads KV head i / (q_heads / kv_heads).
- * F32 queries are served at F32 precision; F16 ones with F32 scores, sums and
- * outputs and weights rounded to f16 once. Rows that see nothing are zeros, rows
+ * F32 queries are served at F32 precision (a weight of the softmax is held to
+ * 2^-22 of itself, or 2^-32 of the row's sum where that is more); F16 ones with F32
+ * scores, sums and outputs and weights rounded to f16 once (2^-11). Rows that see nothing are zeros, rows
  * that see a token with a query that is not finite NaN;
  * positions on a page outside [0, pages) are not attended to; lengths past the
  * table are cut to it; rows of `out` that no sequence has stay as they are. */

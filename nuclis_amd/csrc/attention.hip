@@ -17,10 +17,11 @@
 //
 // Precision. The cache's values are f16 numbers, so K and V enter exactly.
 // F16 queries enter exactly too, and P is rounded to f16 once (a relative
-// 2^-12 of each weight, as large as the rounding of the F16 output). F32
+// 2^-11 of each weight, as large as the rounding of the F16 output). F32
 // queries are carried as two f16 parts after scaling each row by a power of two
-// (22 bits at any magnitude), and P as two parts as well, so outputs keep F32
-// precision. Scores, maxima, sums and outputs are F32. P is kept within
+// (22 bits at any magnitude), and P as two parts as well: 22 bits of each weight, or
+// 2^-32 of the row's sum where that is more, f16's smallest step against the
+// 2^RAISE of the row's largest weight. Scores, maxima, sums and outputs are F32. P is kept within
 // [0, 2^15] relative to a reference that follows the row's maximum: it moves
 // only when a score passes it by 2^8, so most steps rescale nothing.
 //
