@@ -413,7 +413,9 @@ template <int BITS, int D, int RT, bool F32> struct Rows {
             }
     }
     // Scores of the tokens first .. first + 3 (this lane's) that a row does not see become -inf.
-    // (Bitwise on purpose: one select a score, no branches.)
+    // (Bitwise on purpose: one select a score, no branches. Written as `if (!valid || ... || ...) x = -inf`, a
+    // uniform condition before two of the lanes', the compiler leaves the last score's move of a tile in the
+    // uniform condition's block alone; the lanes' own block is empty, and they keep what they should not see.)
     __device__ __forceinline__ void mask(floatx4 (&x)[RT], int first, bool valid) const {
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
