@@ -92,7 +92,9 @@ void nuq_destroy(nuq_context *ctx);
  * be alive when this is called (an event is recorded on it). */
 int nuq_set_stream(nuq_context *ctx, void *stream);
 /* The context's device workspace (verify K-range partials, split partial
- * tiles, the f16 copy of F32 activations, a mixed SiLU pair's second GEMV) is
+ * tiles, the f16 copy of F32 activations, a mixed SiLU pair's second GEMV, the
+ * partial results of an attention whose axis is split, up to 256 MiB, and of a split
+ * row of log probabilities) is
  * allocated on the first call that wants it and grown by powers of two (4 to
  * 512 MiB; nuq_reserve_workspace exactly); nuq_create allocates none. A call
  * that would grow it while a graph capture is active takes its no-workspace
@@ -258,9 +260,9 @@ int nuq_cache_read(nuq_context *ctx, const nuq_cache *cache, const int64_t *slot
  * 16-byte aligned rows; query head i reads KV head i / (q_heads / kv_heads).
  * F32 queries are served at F32 precision (a weight of the softmax is held to
  * 2^-22 of itself, or 2^-32 of the row's sum where that is more); F16 ones with F32
- * scores, sums and outputs and weights rounded to f16 once (2^-11). Rows that see nothing are zeros, rows
- * that see a token with a query that is not finite NaN;
- * positions on a page outside [0, pages) are not attended to; lengths past the
+ * scores, sums and outputs and weights rounded to f16 once (2^-11). Rows that see
+ * nothing are zeros, rows that see a token with a query that is not finite NaN.
+ * Positions on a page outside [0, pages) are not attended to; lengths past the
  * table are cut to it; rows of `out` that no sequence has stay as they are. */
 typedef struct nuq_attention {
     const void *q;

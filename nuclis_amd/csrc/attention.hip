@@ -29,15 +29,18 @@
 // sequence's start) are written as zeros. Positions on a page outside
 // [0, pages) are not attended to.
 //
-// Work split. The four waves of a workgroup take steps of 32 tokens in turn and
-// are merged in LDS; a long axis with few rows is split over workgroups, whose
-// partial (maximum, sum, output) go to the workspace for a second kernel.
+// Work split. The four waves of a workgroup take steps of 32 tokens (16 where two
+// steps of 32 do not fit the registers, step_tiles) in turn and are merged in LDS; a
+// long axis with few rows is split over workgroups, whose partial (maximum, sum,
+// output) go to the workspace for a second kernel.
 //
-// Measured (48 query heads of 128 over 8, 4 bits). One F32 token after 300 tokens:
-// 6.6 us, a chain of four trips to memory; after 32768: 13.7 us and 3.8 for the
-// second kernel (37.8 MB, 7.8 us at a copy's rate). 32 sequences of one F16 token up to
-// 16384: 69 and 4.7 us, 4.6 TB/s, with the vector units half busy. 4 x 8 F32 tokens up
-// to 8191 at 8 bits: 20.6 and 4.0 us, latency and the decode of two blocks of rows.
+// Measured (48 query heads of 128 over 8, 4 bits), kernel by kernel in a trace. One F32
+// token after 300 tokens: 7.0 us, a chain of four trips to memory; after 32768: 14.1 us and 3.9
+// for the second kernel (37.8 MB, which a plain stream of that size reads in 7.1 us; a call among
+// others takes 15.4, so part of a traced kernel's start and end is hidden there). 32 sequences of
+// one F16 token up to 16384: 69 and 4.7 us, 4.6 TB/s in all, with the vector units half busy
+// (F32 78 us a call). 4 x 8 F32 tokens up to 8191 at 8 bits: 24.3 and 4.0 us (25.4 a call, F16 20.9),
+// latency and the decode of two blocks of rows.
 #include "attention_tiles.h"
 
 #include <algorithm>
@@ -412,8 +415,8 @@ static void fit_splits(uint64_t splits, uint64_t rows, uint32_t kv_heads, uint32
 //
 // A batch of both, single tokens among prompts, is two plans where its other sequences
 // are short (at most 256 rows each beside the longest): up to 64 rows by rows, the
-// others by the prompt kernel (a prompt of 512 among 32 single tokens after 8000: 120 us, all
-// by the prompt kernel 738; calls of their own, which know each other's lengths, 78).
+// others by the prompt kernel (a prompt of 512 among 32 single tokens after 8000: 112 us, all
+// by the prompt kernel 738; two calls, which know each kind's lengths, 17 and 68).
 bool plan_attention(uint32_t head_dim, uint32_t kv_heads, uint32_t f32, uint64_t max_length, uint32_t heads,
                     uint64_t max_floats, uint32_t cus, AttentionArgs *a, AttentionArgs *few) {
     max_floats = std::min<uint64_t>(max_floats, 1ull << 26);  // 256 MiB of a call's partial results

@@ -16,7 +16,7 @@
 // Q and a step's scores), since one's products then run under the other's softmax.
 // Operands are read from LDS ahead of their use.
 //
-// Measured (4096 tokens, 48 query heads of 128 over 8, F16, 4 bits): 238 us, 866
+// Measured (4096 tokens, 48 query heads of 128 over 8, F16, 4 bits): 239 us, 862
 // TFLOP/s where a large f16 product reaches 1145 on the same card. The products alone
 // take 153 us, the softmax adds 46 and the decode 53: what bounds it is the vector
 // instructions between products (377 to 96 products a wave's step) that two waves

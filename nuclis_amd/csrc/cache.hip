@@ -9,11 +9,12 @@
 //
 // Memory bound: per token-head 2 D values on one side and D (4 bits + 2) / 16 bytes on
 // the other. The heads of a token are neighbours in the grid, as their values are in
-// memory. Read values go out past the caches in whole lines (32768 tokens of 8 heads of
-// 128, 4 bits: F16 29 us, 6.0 TB/s, 41 with ordinary stores; F32 47, 6.5 TB/s, and 84; with
-// a product that reads them right behind it 75 and 69, 140 and 148: F16 gives that much
-// back there). Writing the same takes 44 us (3.9 TB/s) and 60 us (5.1): about 300 vector
-// instructions a wave of 512 values of each plane, as long as the memory takes.
+// memory. Read values go out past the caches in whole lines. 32768 tokens of 8 heads of
+// 128, 4 bits: F16 25 us, 6.8 TB/s, F32 46 us, 6.6 TB/s (8 bits 30 and 50 us). Calls right
+// behind each other: F16 29 us, 41 with ordinary stores, F32 47 and 75; with a product that
+// reads the values behind each, F16 75 and 70 (so much of it comes back there), F32 140 and
+// 151. Writing the same takes 38 us (4.5 TB/s) and 58 us (5.3), at 8 bits 45 and 65: about 300
+// vector instructions a wave of 512 values of each plane, as long as the memory takes.
 #include "cache.h"
 #include "kernels.h"
 

@@ -17,14 +17,15 @@
 // waves' queues, cut by the last bound, are ranked by counting.
 //
 // Bound by the read of the logits: 1024 rows of 151936 F32 logits with five
-// alternatives take 107 us, 5.8 TB/s (without alternatives 103; as F16 67). The
-// next step's loads are on the way during a step's work, past the caches (118 us
+// alternatives take 99 us, 6.3 TB/s (without alternatives 97; as F16 64). The
+// next step's loads are on the way during a step's work, past the caches (111 us
 // with ordinary loads: nothing is read twice). Each wave with a bound of its own
-// took 161 us: three times the steps looked at single logits.
+// took half as long again: three times the steps looked at single logits.
 // A row is split over workgroups where there are few rows, a step each at the
 // least; the splits' results go to the workspace for a second kernel. One row
-// takes 11 us with twenty alternatives, 64 rows 23 us: a split has a few steps and
-// they all find candidates, then comes the second kernel's 4 us.
+// takes 11 us with twenty alternatives, 64 rows 22 us: a split has a few steps, and
+// its candidates are queued from the first on, before a bound is worth anything; then
+// comes the second kernel's 4 us.
 #include "kernels.h"
 
 namespace nuq {
