@@ -22,7 +22,7 @@ def test_no_divergent_block_is_empty(source, tmp_path):
     assert empty_blocks(asm) == []
 
 
-def test_the_checker_sees_a_dropped_move():
+def test_a_dropped_move_is_seen():
     def blocks(*body):
         return empty_blocks("_ZN3nuq6kernelE:  ; @k\n" + "\n".join(body) + "\n")
 
